@@ -213,9 +213,9 @@ _lib = None
 
 
 def build(force: bool = False) -> str:
-    """Compile the HIP library for gfx950 in-tree (hipcc cross-compiles without a GPU)."""
+    """Compile the HIP library for gfx950 in-tree (hipcc cross-compiles without a GPU).  force: every file, whatever is built."""
     if force or not os.path.exists(LIB_PATH) or _stale():
-        subprocess.check_call(["make", "-C", CSRC, "-j4"], stdout=subprocess.DEVNULL)
+        subprocess.check_call(["make", "-C", CSRC, "-j8"] + (["-B"] if force else []), stdout=subprocess.DEVNULL)
     return LIB_PATH
 
 
