@@ -26,7 +26,7 @@ extern "C" {
 
 #define NR_EINVAL (-1)
 #define NR_MAX_LAYERS 8
-#define NR_ABI_VERSION 28
+#define NR_ABI_VERSION 29
 #define NR_DTYPE_F32 0
 #define NR_DTYPE_BF16 1
 #define NR_DTYPE_F16 2
@@ -890,6 +890,29 @@ int nr_appearance_concat_fwd(const float* features, int n_channels, const float*
 int nr_appearance_concat_bwd(const float* grad_out, int n_channels, int app_dim, const float* times, const int64_t* sensor_idx,
                              float duration, int embeds_per_sensor, int64_t row0, int64_t n_rows, float* grad_features,
                              float* grad_table, int64_t table_rows, nr_stream_t stream);
+/* ------------------------------------------------------------------------------------------------
+ * Embedding rows (v29): a table looked up by index -- per-image or per-sensor embeddings (field_components/embedding.py), class
+ * or token tables -- and its gradient by SORTED indices: no atomics, the same bits on every call, a frequent index spread over
+ * as many blocks as its tokens need.
+ *   table     [rows, dim] of `dtype` (NR_DTYPE_*), rows `row_stride` elements apart; any alignment of that type
+ *   idx       [n] int32 (idx_bytes 4) or int64 (8)
+ *   nr_embedding_fwd   out[i*out_stride + c] = round(scale * table[idx[i], c]); an index outside [0, rows) reads nothing and
+ *                      gives a row of NaN
+ *   nr_embedding_bwd   grad_table[v, c] = round(scale * sum of grad[i, c] over idx[i] == v), sums in fp32 and rounded once;
+ *                      accumulate != 0: round(grad_table[v, c] + that) on the rows looked up, the others untouched; 0: the
+ *                      others are zero.  Indices equal to `padding` (-1: none) or outside [0, rows) contribute nothing.
+ *                      grad: rows grad_stride >= 0 elements apart (0: one row for all).  grad_table: contiguous.
+ *   workspace          nr_embedding_bwd_workspace_bytes(...) bytes, 256-byte aligned, contents irrelevant before and after
+ * dim <= 65 536, rows < 2^31 - 1, n < 2^31 (NR_EINVAL otherwise).  n = 0: nothing is read; a gradient that is not accumulated is
+ * all zero.
+ * ---------------------------------------------------------------------------------------------- */
+int nr_embedding_fwd(const void* table, int dtype, int64_t rows, int dim, int64_t row_stride, const void* idx, int idx_bytes,
+                     int64_t n, float scale, void* out, int64_t out_stride, nr_stream_t stream);
+int64_t nr_embedding_bwd_workspace_bytes(int64_t rows, int dim, int64_t n, int grad_dtype);
+int nr_embedding_bwd(const void* grad, int grad_dtype, int64_t grad_stride, const void* idx, int idx_bytes, int64_t n,
+                     int64_t rows, int dim, float scale, int64_t padding, void* grad_table, int table_dtype, int accumulate,
+                     void* workspace, nr_stream_t stream);
+
 /* Losses of the lidar decoder's two outputs y [n,2] (models/neuradar.py:432-452,624-636 with the multipliers of :690-700):
  * intensity_mult * mean over RETURNING rays of (sigmoid(y0) - target_intensity)^2 (inv_n_returning: device scalar, 1 / their
  * number) + ray_drop_mult * mean BCE-with-logits(y1, !did_return).  The reference additionally masks by the 95 % quantile of
@@ -948,6 +971,29 @@ int nr_adam_hyper(float* step_t, float* dev_hyper, float lr, float lr_final, int
  * nr_amp_update recorded as skipped is not counted -- the scheduler's when ANY group was skipped (the reference steps its
  * schedulers only if the scale did not decrease, engine/trainer.py:590-594), the optimizer's own when ITS step was skipped
  * (torch.optim.Adam's `step` counts performed updates). */
+
+/* ------------------------------------------------------------------------------------------------
+ * Global norm of a list of gradients and their clipping (v29): torch.nn.utils.clip_grad_norm_, which the reference's optimizers
+ * call with their `max_norm` (engine/optimizers.py).  Any number of tensors of any sizes in fp32 / bf16 / fp16; `grads`, `outs`,
+ * `numel`, `dtypes` are HOST arrays of `count` entries (read during the call only: their contents travel as kernel arguments, a
+ * captured graph keeps them); the tensors are dense and aligned to their type.
+ *   nr_grad_norm    result[0] = (sum x^2)^(1/2) (norm_type 2), sum |x| (1) or max |x| (0) over all elements, sums in fp64 in a fixed
+ *                   order; result[1] = min(1, max_norm / (result[0] + 1e-6)), NaN if the norm is.  max_norm >= 0 (infinity: a
+ *                   factor of 1).  NaN and infinities of the gradients reach the norm.  No elements: norm 0.
+ *   nr_grad_scale   outs[t] = round(result[1] * grads[t]); outs[t] == grads[t] is in place, and then a factor of 1 moves nothing
+ *   workspace       nr_grad_norm_workspace_bytes(numel, count) bytes, 8-byte aligned
+ * nr_adam_step_clipped: nr_adam_step with the gradient multiplied by clip[0] (device float; result + 1 of nr_grad_norm) besides
+ * grad_scale -- clipping inside the optimizer's own pass, the gradients are not rewritten for it.
+ * ---------------------------------------------------------------------------------------------- */
+int64_t nr_grad_norm_workspace_bytes(const int64_t* numel, int count);
+int nr_grad_norm(const void* const* grads, const int64_t* numel, const int32_t* dtypes, int count, int norm_type, double max_norm,
+                 float* result, void* workspace, nr_stream_t stream);
+int nr_grad_scale(const void* const* grads, void* const* outs, const int64_t* numel, const int32_t* dtypes,
+                  const int32_t* out_dtypes, int count, const float* result, nr_stream_t stream);
+int nr_adam_step_clipped(float* param, float* grad, float* exp_avg, float* exp_avg_sq, int64_t n,
+                         float lr, float beta1, float beta2, float eps, float weight_decay, int adamw,
+                         int step, float grad_scale, int zero_grad, const float* dev_hyper, uint8_t* seen_grad,
+                         const float* skip, void* delta16, int state_stride, const float* clip, nr_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------------
  * Dynamic loss scale with found-inf guard: torch.cuda.amp.GradScaler (engine/trainer.py:200,572-594;

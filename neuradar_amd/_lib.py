@@ -7,14 +7,14 @@ __graft_entry__ as g; g.build()"` or `make -C neuradar_amd/csrc`).
 import ctypes
 import os
 import subprocess
-from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int64, c_uint32, c_void_p
+from ctypes import POINTER, Structure, c_char_p, c_double, c_float, c_int, c_int64, c_uint32, c_void_p
 
 CSRC = os.path.join(os.path.dirname(os.path.abspath(__file__)), "csrc")
 LIB_PATH = os.environ.get("NR_LIB_PATH") or os.path.join(CSRC, "libneuradar_hip.so")  # (NR_LIB_PATH: A/B runs of two builds)
 NR_MAX_LAYERS = 8
 NR_EINVAL = -1
 NR_LOSS_SLOTS = 1024
-NR_ABI_VERSION = 28
+NR_ABI_VERSION = 29
 NR_DTYPES = {"float32": 0, "bfloat16": 1, "float16": 2}  # nr_field_t.dtype
 # nr_amp state layout (include/neuradar_hip.h)
 NR_AMP_MAX_GROUPS, NR_AMP_SCALE, NR_AMP_GROWTH_TRACKER, NR_AMP_INV_SCALE, NR_AMP_SKIPPED_PREV, NR_AMP_SKIPPED_TOTAL = 8, 0, 1, 2, 3, 4
@@ -77,7 +77,7 @@ class NrFieldGrads(Structure):
     _fields_ = [("geo", NrMlpGrads), ("feat", NrMlpGrads), ("beta", c_void_p)]
 
 
-P, I, L, F = c_void_p, c_int, c_int64, c_float
+P, I, L, F, D = c_void_p, c_int, c_int64, c_float, c_double
 
 # name -> argtypes (return type is int unless listed in _RESTYPES).  Mirrors include/neuradar_hip.h.
 PROTOTYPES = {
@@ -172,6 +172,9 @@ PROTOTYPES = {
     "nr_lidar_losses": [P, P, POINTER(NrLidarLosses), P, P, P, P, P, P],
     "nr_appearance_concat_fwd": [P, I, P, I, P, P, F, I, L, L, P, P],
     "nr_appearance_concat_bwd": [P, I, I, P, P, F, I, L, L, P, P, L, P],
+    "nr_embedding_fwd": [P, I, L, I, L, P, I, L, F, P, L, P],
+    "nr_embedding_bwd_workspace_bytes": [L, I, L, I],
+    "nr_embedding_bwd": [P, I, L, P, I, L, L, I, F, L, P, I, I, P, P],
     "nr_lidar_head_loss": [P, P, P, L, P, F, F, P, P, P],
     "nr_depth_from_weights": [P, P, L, I, P, P],
     "nr_gen_rays_camera": [P, P, P, P, P, P, P, P, P, P, P, P, L, P, P, P, P, P, P],
@@ -181,6 +184,10 @@ PROTOTYPES = {
     "nr_permutation_from_uniform": [P, I, P, P],
     "nr_gen_rays_radar": [P, L, P, P, F, F, I, F, F, I, P, P, P, P, P, P],
     "nr_adam_step": [P, P, P, P, L, F, F, F, F, F, I, I, F, I, P, P, P, P, I, P],
+    "nr_grad_norm_workspace_bytes": [P, I],
+    "nr_grad_norm": [P, P, P, I, I, D, P, P, P],
+    "nr_grad_scale": [P, P, P, P, P, I, P, P],
+    "nr_adam_step_clipped": [P, P, P, P, L, F, F, F, F, F, I, I, F, I, P, P, P, P, I, P, P],
     "nr_apply_delta16": [P, P, L, L, L, P],
     "nr_grad_to16_clear": [P, P, L, P],
     "nr_adam_step_marked": [P, P, P, P, L, F, F, F, F, I, F, I, P, P, P, I, P],
@@ -206,6 +213,7 @@ _RESTYPES = {"nr_target_arch": c_char_p, "nr_param_generation": c_void_p, "nr_fi
              "nr_field_stash_floats": c_int64, "nr_hash_encode_bwd_binned_workspace_bytes": c_int64,
              "nr_tcnn_grid_param_count": c_int64, "nr_attention_workspace_floats": c_int64,
              "nr_radar_assign_workspace_bytes": c_int64, "nr_radar_assign_status_offset": c_int64,
+             "nr_embedding_bwd_workspace_bytes": c_int64, "nr_grad_norm_workspace_bytes": c_int64,
              "nr_bn_act_workspace_floats": c_int64, "nr_conv7_image_bytes": c_int64,
              "nr_conv7_wgrad_workspace_bytes": c_int64, "nr_pw_workspace_bytes": c_int64}
 

@@ -1,0 +1,565 @@
+// Rows of an embedding table, and the table's gradient.
+//
+//   rows      out[i, :] = round(scale * table[idx[i], :])                                     (nr_embedding_fwd)
+//   gradient  g_table[v, :] (+)= round(scale * sum over i with idx[i] = v of g[i, :])         (nr_embedding_bwd)
+//
+// The gradient is a sum over equal indices.  Adding rows to the table as they come needs float atomics, whose order -- and with
+// it the result -- changes from run to run, and a row that many tokens share becomes one queue at the memory side.  Here the
+// (index, position) pairs are SORTED first (stable, so equal indices keep their positions in ascending order); then equal
+// indices are neighbours, every sum is formed in registers in one fixed order, and each touched row is written once.
+//   * sort: least significant digit first, digits of up to 11 bits (one pass for 2 047 rows, two for 4 M); per pass a count, a
+//     scan and a scatter.  Indices that get no gradient (padding, out of range) take the key `rows` and end up last.
+//   * sum: a block takes a fixed stretch of SORTED positions, whatever the indices are -- a row that owns half of the batch is
+//     spread over as many blocks as its tokens need.  Groups of lanes walk shorter stretches, U rows of g in flight each; a sum
+//     whose neighbours lie in other stretches goes through LDS to its first group, one that leaves the block is left in the
+//     workspace.
+//   * join: sums that cross blocks are added up in block order by the block they start in.
+// All sums are held in fp32; the order is that of the stretches, fixed by (n, dim) alone: two calls give the same bits.
+#include "rows_dev.h"
+
+namespace {
+
+constexpr int kMaxDim = 65536;
+constexpr int kThreads = 256;
+constexpr int kRounds = 8;                            // rounds of 64 tokens that a wave ranks in one tile of the sort
+constexpr int kTile = kThreads * kRounds;             // tokens per block of the sort
+constexpr int kMaxDigitBits = 11;
+
+// ---------------------------------------------------------------------------------------------------------------- rows
+constexpr int kRowUnroll = 4;
+
+// Flat over the 16-byte vectors of the output, four per thread: every lane has work whatever the width is.  A row's last vector
+// may be short (dim not a multiple of the vector): element by element.
+template <typename T, typename I>
+__global__ void __launch_bounds__(kThreads)
+rows_kernel(const T* __restrict__ table, int64_t rows, int dim, int64_t row_stride, const I* __restrict__ idx, int64_t n, float scale,
+            T* __restrict__ out, int64_t out_stride, uint32_t nv, uint32_t magic) {
+  constexpr int N = 16 / (int)sizeof(T);
+  const int64_t base = (int64_t)blockIdx.x * (kThreads * kRowUnroll);
+  const int64_t row0 = base / nv;
+  const uint32_t rem0 = (uint32_t)(base - row0 * nv);
+  int64_t r[kRowUnroll], v[kRowUnroll];
+  int col[kRowUnroll];
+#pragma unroll
+  for (int u = 0; u < kRowUnroll; ++u) {
+    const uint32_t l = rem0 + (uint32_t)(u * kThreads) + threadIdx.x;
+    const uint32_t q = magic == 0u ? l : __umulhi(l, magic);
+    r[u] = row0 + q;
+    col[u] = (int)(l - q * nv) * N;
+    v[u] = r[u] < n ? (int64_t)idx[r[u]] : -1;
+  }
+  float x[kRowUnroll][N];
+#pragma unroll
+  for (int u = 0; u < kRowUnroll; ++u) {
+    if (v[u] >= 0 && v[u] < rows) {
+      nr_load_some<T, N>(table + v[u] * row_stride + col[u], dim - col[u], x[u]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < N; ++k) x[u][k] = __builtin_nanf("");
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kRowUnroll; ++u) {
+    if (r[u] >= n) continue;
+#pragma unroll
+    for (int k = 0; k < N; ++k) x[u][k] *= scale;
+    nr_store_some<T, N>(out + r[u] * out_stride + col[u], dim - col[u], x[u]);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- sort
+struct SortPass {
+  const uint32_t* keys;   // NULL: this pass reads the indices themselves
+  const uint32_t* pos;
+  uint32_t* keys_out;
+  uint32_t* pos_out;
+  uint32_t* counts;       // [digits][blocks]
+  uint32_t* totals;       // [digits]
+  int64_t n, rows, padding;
+  int shift, bits;
+  uint32_t blocks;
+};
+
+template <typename I>
+__device__ __forceinline__ uint32_t key_of(const SortPass& s, const I* __restrict__ idx, int64_t i) {
+  if (s.keys != nullptr) return s.keys[i];
+  const int64_t v = (int64_t)idx[i];
+  return (v >= 0 && v < s.rows && v != s.padding) ? (uint32_t)v : (uint32_t)s.rows;
+}
+
+template <typename I>
+__global__ void __launch_bounds__(kThreads)
+sort_count_kernel(SortPass s, const I* __restrict__ idx) {
+  __shared__ uint32_t cnt[1 << kMaxDigitBits];
+  const int digits = 1 << s.bits;
+  for (int d = threadIdx.x; d < digits; d += kThreads) cnt[d] = 0u;
+  __syncthreads();
+  const int64_t base = (int64_t)blockIdx.x * kTile;
+#pragma unroll
+  for (int u = 0; u < kRounds; ++u) {
+    const int64_t i = base + u * kThreads + threadIdx.x;
+    if (i < s.n) atomicAdd(&cnt[(key_of(s, idx, i) >> s.shift) & (uint32_t)(digits - 1)], 1u);
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < digits; d += kThreads) s.counts[(int64_t)d * s.blocks + blockIdx.x] = cnt[d];
+}
+
+// counts[d][b] -> tokens of digit d in blocks before b; totals[d].  One wave per digit.
+__global__ void __launch_bounds__(kThreads)
+sort_scan_kernel(SortPass s) {
+  const int d = (int)(blockIdx.x * (kThreads / NR_WAVE) + threadIdx.x / NR_WAVE);
+  if (d >= (1 << s.bits)) return;
+  const int lane = nr_lane();
+  uint32_t* c = s.counts + (int64_t)d * s.blocks;
+  uint32_t before = 0u;
+  for (uint32_t b0 = 0; b0 < s.blocks; b0 += NR_WAVE) {
+    const uint32_t b = b0 + lane;
+    const uint32_t own = b < s.blocks ? c[b] : 0u;
+    uint32_t incl = own;
+#pragma unroll
+    for (int o = 1; o < NR_WAVE; o <<= 1) {
+      const uint32_t t = __shfl_up(incl, o, NR_WAVE);
+      if (lane >= o) incl += t;
+    }
+    if (b < s.blocks) c[b] = before + incl - own;
+    before += __shfl(incl, NR_WAVE - 1, NR_WAVE);
+  }
+  if (lane == 0) s.totals[d] = before;
+}
+
+// Exclusive prefix sums of x[0 .. count) in LDS by the whole block; scratch: kThreads words.
+__device__ __forceinline__ void block_exclusive_scan(uint32_t* x, int count, uint32_t* scratch) {
+  const int per = (count + kThreads - 1) / kThreads, lo = threadIdx.x * per;
+  uint32_t sum = 0u;
+  for (int k = 0; k < per; ++k)
+    if (lo + k < count) sum += x[lo + k];
+  scratch[threadIdx.x] = sum;
+  __syncthreads();
+  for (int o = 1; o < kThreads; o <<= 1) {
+    const uint32_t t = (int)threadIdx.x >= o ? scratch[threadIdx.x - o] : 0u;
+    __syncthreads();
+    scratch[threadIdx.x] += t;
+    __syncthreads();
+  }
+  uint32_t run = scratch[threadIdx.x] - sum;
+  for (int k = 0; k < per; ++k)
+    if (lo + k < count) {
+      const uint32_t own = x[lo + k];
+      x[lo + k] = run;
+      run += own;
+    }
+  __syncthreads();
+}
+
+// A wave ranks 64 tokens at a time: lanes of equal digit find each other by one ballot per bit, the lowest of them advances the
+// wave's counter by their number.  Waves own consecutive quarters of the tile, so the order of equal digits is kept.
+template <typename I>
+__global__ void __launch_bounds__(kThreads)
+sort_scatter_kernel(SortPass s, const I* __restrict__ idx) {
+  constexpr int kWaves = kThreads / NR_WAVE;
+  __shared__ uint32_t cnt[kWaves][1 << kMaxDigitBits];
+  __shared__ uint32_t first[1 << kMaxDigitBits];
+  __shared__ uint32_t scratch[kThreads];
+  const int digits = 1 << s.bits, lane = nr_lane(), wave = threadIdx.x / NR_WAVE;
+  for (int d = threadIdx.x; d < digits; d += kThreads) {
+    first[d] = s.totals[d];
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) cnt[w][d] = 0u;
+  }
+  __syncthreads();
+  const int64_t base = (int64_t)blockIdx.x * kTile + (int64_t)wave * (NR_WAVE * kRounds);
+  uint32_t key[kRounds], pos[kRounds], rank[kRounds];
+#pragma unroll
+  for (int u = 0; u < kRounds; ++u) {
+    const int64_t i = base + u * NR_WAVE + lane;
+    const bool in = i < s.n;
+    key[u] = in ? key_of(s, idx, i) : 0u;
+    pos[u] = in ? (s.pos != nullptr ? s.pos[i] : (uint32_t)i) : 0u;
+  }
+#pragma unroll
+  for (int u = 0; u < kRounds; ++u) {
+    const bool in = base + u * NR_WAVE + lane < s.n;
+    const uint32_t d = (key[u] >> s.shift) & (uint32_t)(digits - 1);
+    uint64_t peers = __ballot(in);
+    for (int b = 0; b < s.bits; ++b) {
+      const uint64_t ones = __ballot((d >> b) & 1u);
+      peers &= ((d >> b) & 1u) ? ones : ~ones;
+    }
+    const int leader = in ? __ffsll((unsigned long long)peers) - 1 : lane;
+    uint32_t old = 0u;
+    if (in && lane == leader) old = atomicAdd(&cnt[wave][d], (uint32_t)__popcll(peers));
+    old = __shfl(old, leader, NR_WAVE);
+    rank[u] = old + (uint32_t)__popcll(peers & ((1ull << lane) - 1ull));
+  }
+  __syncthreads();
+  block_exclusive_scan(first, digits, scratch);
+  for (int d = threadIdx.x; d < digits; d += kThreads) {
+    uint32_t at = first[d] + s.counts[(int64_t)d * s.blocks + blockIdx.x];
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const uint32_t own = cnt[w][d];
+      cnt[w][d] = at;
+      at += own;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < kRounds; ++u) {
+    if (base + u * NR_WAVE + lane >= s.n) continue;
+    const uint32_t to = cnt[wave][(key[u] >> s.shift) & (uint32_t)(digits - 1)] + rank[u];
+    s.keys_out[to] = key[u];
+    s.pos_out[to] = pos[u];
+  }
+}
+
+// ----------------------------------------------------------------------------------------------------------------- sum
+struct SumArgs {
+  const uint32_t* keys;  // sorted
+  const uint32_t* pos;
+  int64_t n, rows;
+  int dim;
+  int64_t grad_stride;
+  float scale;
+  void* out;
+  int out_dtype, accumulate;
+  float* head;      // [blocks][dim]: the part of a sum that started in an earlier block
+  float* tail;      // [blocks][dim]: the part of a sum that goes on in the next one
+  uint32_t* flags;  // [blocks]: kHead | kSpan | kTail
+  int group, groups, per_group;  // lanes per row, rows at a time, sorted positions per group
+};
+constexpr uint32_t kHead = 1u, kSpan = 2u, kTail = 4u;
+
+template <int N, typename O>
+__device__ __forceinline__ void write_row_as(const SumArgs& a, uint32_t row, int col, float (&x)[N]) {
+  O* o = static_cast<O*>(a.out) + (int64_t)row * a.dim + col;
+#pragma unroll
+  for (int k = 0; k < N; ++k) x[k] *= a.scale;
+  if (a.accumulate) {
+    float was[N];
+    nr_load_some<O, N>(o, a.dim - col, was);
+#pragma unroll
+    for (int k = 0; k < N; ++k) x[k] += was[k];
+  }
+  nr_store_some<O, N>(o, a.dim - col, x);
+}
+template <int N>
+__device__ __forceinline__ void write_row(const SumArgs& a, uint32_t row, int col, float (&x)[N]) {
+  if (a.out_dtype == NR_DTYPE_F32) write_row_as<N, float>(a, row, col, x);
+  else if (a.out_dtype == NR_DTYPE_BF16) write_row_as<N, __bf16>(a, row, col, x);
+  else write_row_as<N, _Float16>(a, row, col, x);
+}
+
+constexpr int kMaxStretch = 4096;  // sorted positions of one block (32 KB of LDS)
+constexpr int kFlight = 8;  // rows of g requested before the first of them is added
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+sum_kernel(SumArgs a, const T* __restrict__ grad) {
+  constexpr int N = 16 / (int)sizeof(T);
+  extern __shared__ uint32_t lds[];
+  const int per_block = a.groups * a.per_group;
+  uint32_t* s_key = lds;                            // [per_block + 2]: the keys before, in and behind the stretch
+  uint32_t* s_pos = s_key + per_block + 2;          // [per_block]
+  uint32_t* s_flag = s_pos + per_block;             // [groups]
+  uint32_t* s_left = s_flag + a.groups;             // [groups]: what a group leaves for the blocks around this one
+  float* s_head = reinterpret_cast<float*>(s_left + a.groups);  // [groups][group * N]
+  float* s_tail = s_head + a.groups * a.group * N;
+  const int64_t p0 = (int64_t)blockIdx.x * per_block;
+  constexpr uint32_t kNone = 0xFFFFFFFFu;
+  for (int i = threadIdx.x; i < per_block + 2; i += kThreads) {
+    const int64_t p = p0 + i - 1;
+    s_key[i] = (p >= 0 && p < a.n) ? a.keys[p] : kNone;
+    if (i >= 1 && i <= per_block) s_pos[i - 1] = p < a.n ? a.pos[p] : 0u;
+  }
+  __syncthreads();
+  const int r = threadIdx.x / a.group, lane = threadIdx.x - r * a.group;
+  const int col = (blockIdx.y * a.group + lane) * N;
+  const bool work = r < a.groups && col < a.dim;
+  const uint32_t ignored = (uint32_t)a.rows;
+  float acc[N];
+  if (work) {
+    const int q0 = r * a.per_group;
+    uint32_t flag = 0u;
+    bool open_here = s_key[q0] != s_key[q0 + 1];  // does the first sum start in this stretch?
+#pragma unroll
+    for (int k = 0; k < N; ++k) acc[k] = 0.0f;
+    for (int q = q0; q < q0 + a.per_group; q += kFlight) {
+      float x[kFlight][N];
+#pragma unroll
+      for (int u = 0; u < kFlight; ++u) {
+        if (q + u < q0 + a.per_group && s_key[q + u + 1] < ignored) {
+          nr_load_some<T, N>(grad + (int64_t)s_pos[q + u] * a.grad_stride + col, a.dim - col, x[u]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < N; ++k) x[u][k] = 0.0f;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kFlight; ++u) {
+        const int at = q + u;
+        if (at >= q0 + a.per_group) break;
+        const uint32_t key = s_key[at + 1], next = s_key[at + 2];
+        if (key >= ignored) break;  // (padding, out of range, behind the end: nothing follows)
+#pragma unroll
+        for (int k = 0; k < N; ++k) acc[k] += x[u][k];
+        const bool last = at + 1 == q0 + a.per_group;
+        if (key != next || last) {
+          const bool goes_on = key == next;
+          float* part = nullptr;
+          if (!open_here) {
+            part = s_head + (r * a.group + lane) * N;
+            flag |= goes_on ? kHead | kSpan : kHead;
+          } else if (goes_on) {
+            part = s_tail + (r * a.group + lane) * N;
+            flag |= kTail;
+          }
+          if (part != nullptr) {
+#pragma unroll
+            for (int k = 0; k < N; ++k) part[k] = acc[k];
+          } else {
+            write_row<N>(a, key, col, acc);
+          }
+          open_here = true;
+#pragma unroll
+          for (int k = 0; k < N; ++k) acc[k] = 0.0f;
+        }
+      }
+    }
+    if (lane == 0) s_flag[r] = flag;
+  }
+  __syncthreads();
+  // sums that cross stretches: their first group adds the parts behind it, in order.  Group 0 also takes a sum that came in
+  // from the block before.
+  if (work) {
+    const uint32_t own = s_flag[r];
+    auto follow = [&](int j) {  // adds the heads of groups j, j + 1, ...; true: the sum ended in this block
+      for (; j < a.groups; ++j) {
+        const float* part = s_head + (j * a.group + lane) * N;
+#pragma unroll
+        for (int k = 0; k < N; ++k) acc[k] += part[k];
+        if ((s_flag[j] & kSpan) == 0u) return true;
+      }
+      return false;
+    };
+    uint32_t flag = 0u;
+    const int64_t slot = (int64_t)blockIdx.x * a.dim + col;
+    if (r == 0 && (own & kHead)) {
+#pragma unroll
+      for (int k = 0; k < N; ++k) acc[k] = 0.0f;
+      flag |= follow(0) ? kHead : kHead | kSpan;
+      nr_store_some<float, N>(a.head + slot, a.dim - col, acc);
+    }
+    if (own & kTail) {
+      const float* part = s_tail + (r * a.group + lane) * N;
+#pragma unroll
+      for (int k = 0; k < N; ++k) acc[k] = part[k];
+      if (follow(r + 1)) {
+        write_row<N>(a, s_key[(r + 1) * a.per_group], col, acc);
+      } else {
+        nr_store_some<float, N>(a.tail + slot, a.dim - col, acc);
+        flag |= kTail;
+      }
+    }
+    if (blockIdx.y == 0 && lane == 0) s_left[r] = flag;
+  }
+  __syncthreads();
+  if (blockIdx.y == 0 && threadIdx.x == 0) {
+    uint32_t flag = 0u;
+    for (int j = 0; j < a.groups; ++j) flag |= s_left[j];
+    a.flags[blockIdx.x] = flag;
+  }
+}
+
+// A sum that starts in block b and leaves it: tail[b] + head[b + 1] + ... + the head that ends it.  One thread per 4 columns,
+// blocks in order.
+__global__ void __launch_bounds__(kThreads)
+join_kernel(SumArgs a, uint32_t blocks) {
+  const uint32_t b = blockIdx.x;
+  if ((a.flags[b] & kTail) == 0u) return;
+  const int64_t per_block = (int64_t)a.groups * a.per_group;
+  const uint32_t key = a.keys[(b + 1) * per_block - 1];
+  for (int col = threadIdx.x * 4; col < a.dim; col += kThreads * 4) {
+    float acc[4], x[4];
+    nr_load_some<float, 4>(a.tail + (int64_t)b * a.dim + col, a.dim - col, acc);
+    for (uint32_t j = b + 1; j < blocks; ++j) {
+      nr_load_some<float, 4>(a.head + (int64_t)j * a.dim + col, a.dim - col, x);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[k] += x[k];
+      if ((a.flags[j] & kSpan) == 0u) break;
+    }
+    write_row<4>(a, key, col, acc);
+  }
+}
+
+__global__ void __launch_bounds__(kThreads)
+clear_kernel(uint16_t* __restrict__ p, int64_t halves) {
+  typedef NrPack<uint16_t, 8> Pack;
+  const int64_t packs = halves / 8;
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < packs; i += (int64_t)gridDim.x * kThreads)
+    reinterpret_cast<Pack*>(p)[i].v = (Pack::vec)(uint16_t)0;
+  if (blockIdx.x == 0)
+    for (int64_t i = packs * 8 + threadIdx.x; i < halves; i += kThreads) p[i] = 0;
+}
+
+// ---------------------------------------------------------------------------------------------------------------- host
+int dtype_size(int dtype) { return dtype == NR_DTYPE_F32 ? 4 : 2; }
+bool dtype_ok(int dtype) { return dtype == NR_DTYPE_F32 || dtype == NR_DTYPE_BF16 || dtype == NR_DTYPE_F16; }
+
+struct Plan {
+  int bits, passes, digit_bits;
+  uint32_t sort_blocks, sum_blocks;
+  int group, groups, per_group, col_tiles;
+  int64_t off_pairs, off_counts, off_totals, off_flags, off_parts, bytes;
+};
+
+// Everything that follows from the sizes: the digits of the sort, the stretches of the sum and the workspace.  The layout takes
+// the narrower vector (4 columns per lane): one size for every type of gradient.
+Plan make_plan(int64_t rows, int dim, int64_t n, int elem_size) {
+  Plan p = {};
+  while ((rows >> p.bits) != 0) ++p.bits;  // keys 0 .. rows
+  p.passes = (p.bits + kMaxDigitBits - 1) / kMaxDigitBits;
+  p.digit_bits = (p.bits + p.passes - 1) / p.passes;
+  p.sort_blocks = (uint32_t)nr_cdiv(n, kTile);
+  const int vec = 16 / elem_size, nv = (dim + vec - 1) / vec;
+  p.col_tiles = (nv + kThreads - 1) / kThreads;
+  p.group = (nv + p.col_tiles - 1) / p.col_tiles;
+  p.groups = kThreads / p.group;
+  p.per_group = 64;
+  while (p.groups * p.per_group > kMaxStretch) p.per_group /= 2;
+  while (p.per_group > kFlight && nr_cdiv(n, (int64_t)p.groups * p.per_group) * p.col_tiles < 1024) p.per_group /= 2;
+  p.sum_blocks = (uint32_t)nr_cdiv(n, (int64_t)p.groups * p.per_group);
+  auto place = [&p](int64_t bytes) {
+    const int64_t at = p.bytes;
+    p.bytes += (bytes + 255) / 256 * 256;
+    return at;
+  };
+  p.off_pairs = place(4 * n * (int64_t)sizeof(uint32_t));
+  p.off_counts = place(((int64_t)1 << p.digit_bits) * p.sort_blocks * (int64_t)sizeof(uint32_t));
+  p.off_totals = place(((int64_t)1 << p.digit_bits) * (int64_t)sizeof(uint32_t));
+  p.off_flags = place((int64_t)p.sum_blocks * (int64_t)sizeof(uint32_t));
+  p.off_parts = place(2 * (int64_t)p.sum_blocks * dim * (int64_t)sizeof(float));
+  return p;
+}
+
+bool sizes_ok(int64_t rows, int dim, int64_t n) {
+  return rows >= 0 && rows <= 0x7FFFFFFE && dim >= 0 && dim <= kMaxDim && n >= 0 && n <= 0x7FFFFFFF;
+}
+
+template <typename T>
+int launch_rows(const void* table, int64_t rows, int dim, int64_t row_stride, const void* idx, int idx_bytes, int64_t n, float scale,
+                void* out, int64_t out_stride, hipStream_t stream) {
+  constexpr int N = 16 / (int)sizeof(T);
+  const uint32_t nv = (uint32_t)((dim + N - 1) / N);
+  // l / nv = umulhi(l, magic) while l * nv < 2^32: l < nv + 1 024, nv <= 16 384
+  const uint32_t magic = nv == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + nv - 1) / nv);
+  const dim3 grid((uint32_t)nr_cdiv(n * nv, kThreads * kRowUnroll));
+  if (idx_bytes == 8)
+    hipLaunchKernelGGL((rows_kernel<T, int64_t>), grid, dim3(kThreads), 0, stream, static_cast<const T*>(table), rows, dim, row_stride,
+                       static_cast<const int64_t*>(idx), n, scale, static_cast<T*>(out), out_stride, nv, magic);
+  else
+    hipLaunchKernelGGL((rows_kernel<T, int32_t>), grid, dim3(kThreads), 0, stream, static_cast<const T*>(table), rows, dim, row_stride,
+                       static_cast<const int32_t*>(idx), n, scale, static_cast<T*>(out), out_stride, nv, magic);
+  NR_LAUNCH_CHECK();
+  return 0;
+}
+
+template <typename I>
+int launch_sort(const Plan& p, SortPass s, const void* idx, uint32_t* const (&pairs)[4], hipStream_t stream) {
+  for (int pass = 0; pass < p.passes; ++pass) {
+    s.shift = pass * p.digit_bits;
+    s.bits = p.digit_bits;
+    s.keys = pass == 0 ? nullptr : pairs[(pass - 1) % 2 * 2];
+    s.pos = pass == 0 ? nullptr : pairs[(pass - 1) % 2 * 2 + 1];
+    s.keys_out = pairs[pass % 2 * 2];
+    s.pos_out = pairs[pass % 2 * 2 + 1];
+    hipLaunchKernelGGL(sort_count_kernel<I>, dim3(p.sort_blocks), dim3(kThreads), 0, stream, s, static_cast<const I*>(idx));
+    hipLaunchKernelGGL(sort_scan_kernel, dim3((uint32_t)nr_cdiv(1 << s.bits, kThreads / NR_WAVE)), dim3(kThreads), 0, stream, s);
+    hipLaunchKernelGGL(sort_scatter_kernel<I>, dim3(p.sort_blocks), dim3(kThreads), 0, stream, s, static_cast<const I*>(idx));
+    NR_LAUNCH_CHECK();
+  }
+  return 0;
+}
+
+template <typename T>
+int launch_sum(const Plan& p, const SumArgs& a, const void* grad, hipStream_t stream) {
+  constexpr int N = 16 / (int)sizeof(T);
+  const int per_block = a.groups * a.per_group;
+  const size_t lds = (size_t)(2 * per_block + 2 + 2 * a.groups + 2 * a.groups * a.group * N) * 4;
+  hipLaunchKernelGGL(sum_kernel<T>, dim3(p.sum_blocks, (uint32_t)p.col_tiles), dim3(kThreads), lds, stream, a, static_cast<const T*>(grad));
+  NR_LAUNCH_CHECK();
+  hipLaunchKernelGGL(join_kernel, dim3(p.sum_blocks), dim3(kThreads), 0, stream, a, p.sum_blocks);
+  NR_LAUNCH_CHECK();
+  return 0;
+}
+
+}  // namespace
+
+extern "C" int nr_embedding_fwd(const void* table, int dtype, int64_t rows, int dim, int64_t row_stride, const void* idx, int idx_bytes,
+                                int64_t n, float scale, void* out, int64_t out_stride, nr_stream_t stream) {
+  if (!dtype_ok(dtype) || !sizes_ok(rows, dim, n) || (idx_bytes != 4 && idx_bytes != 8) || row_stride < 0 || out_stride < dim) return NR_EINVAL;
+  if (n == 0 || dim == 0) return 0;
+  if (idx == nullptr || out == nullptr || (table == nullptr && rows > 0)) return NR_EINVAL;
+  const int vec = 16 / dtype_size(dtype);
+  if (nr_cdiv(n * ((dim + vec - 1) / vec), kThreads * kRowUnroll) > 0x7FFFFFFF) return NR_EINVAL;  // (blocks of one launch)
+  if (dtype == NR_DTYPE_F32) return launch_rows<float>(table, rows, dim, row_stride, idx, idx_bytes, n, scale, out, out_stride, nr_s(stream));
+  if (dtype == NR_DTYPE_BF16) return launch_rows<__bf16>(table, rows, dim, row_stride, idx, idx_bytes, n, scale, out, out_stride, nr_s(stream));
+  return launch_rows<_Float16>(table, rows, dim, row_stride, idx, idx_bytes, n, scale, out, out_stride, nr_s(stream));
+}
+
+extern "C" int64_t nr_embedding_bwd_workspace_bytes(int64_t rows, int dim, int64_t n, int grad_dtype) {
+  if (!dtype_ok(grad_dtype) || !sizes_ok(rows, dim, n)) return NR_EINVAL;
+  if (n == 0 || dim == 0 || rows == 0) return 0;
+  return make_plan(rows, dim, n, dtype_size(grad_dtype)).bytes;
+}
+
+extern "C" int nr_embedding_bwd(const void* grad, int grad_dtype, int64_t grad_stride, const void* idx, int idx_bytes, int64_t n, int64_t rows,
+                                int dim, float scale, int64_t padding, void* grad_table, int table_dtype, int accumulate, void* workspace,
+                                nr_stream_t stream) {
+  if (!dtype_ok(grad_dtype) || !dtype_ok(table_dtype) || !sizes_ok(rows, dim, n) || (idx_bytes != 4 && idx_bytes != 8) || grad_stride < 0)
+    return NR_EINVAL;
+  if (rows == 0 || dim == 0) return 0;
+  if (grad_table == nullptr || (reinterpret_cast<uintptr_t>(grad_table) & (uintptr_t)(dtype_size(table_dtype) - 1)) != 0) return NR_EINVAL;
+  if (n > 0 && (grad == nullptr || idx == nullptr || workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0)) return NR_EINVAL;
+  hipStream_t st = nr_s(stream);
+  if (!accumulate) {
+    // the whole table: rows that nothing looks up are zero
+    const int64_t halves = rows * dim * (dtype_size(table_dtype) / 2);
+    const int64_t blocks = nr_cdiv(halves, kThreads * 8);
+    hipLaunchKernelGGL(clear_kernel, dim3((uint32_t)(blocks < 4096 ? blocks : 4096)), dim3(kThreads), 0, st,
+                       static_cast<uint16_t*>(grad_table), halves);
+    NR_LAUNCH_CHECK();
+  }
+  if (n == 0) return 0;
+  const Plan p = make_plan(rows, dim, n, dtype_size(grad_dtype));
+  char* ws = static_cast<char*>(workspace);
+  uint32_t* pairs[4];
+  for (int k = 0; k < 4; ++k) pairs[k] = reinterpret_cast<uint32_t*>(ws + p.off_pairs) + (int64_t)k * n;
+  SortPass s = {};
+  s.counts = reinterpret_cast<uint32_t*>(ws + p.off_counts);
+  s.totals = reinterpret_cast<uint32_t*>(ws + p.off_totals);
+  s.n = n;
+  s.rows = rows;
+  s.padding = padding;
+  s.blocks = p.sort_blocks;
+  if (int rc = idx_bytes == 8 ? launch_sort<int64_t>(p, s, idx, pairs, st) : launch_sort<int32_t>(p, s, idx, pairs, st)) return rc;
+  SumArgs a = {};
+  a.keys = pairs[(p.passes - 1) % 2 * 2];
+  a.pos = pairs[(p.passes - 1) % 2 * 2 + 1];
+  a.n = n;
+  a.rows = rows;
+  a.dim = dim;
+  a.grad_stride = grad_stride;
+  a.scale = scale;
+  a.out = grad_table;
+  a.out_dtype = table_dtype;
+  a.accumulate = accumulate;
+  a.flags = reinterpret_cast<uint32_t*>(ws + p.off_flags);
+  a.head = reinterpret_cast<float*>(ws + p.off_parts);
+  a.tail = a.head + (int64_t)p.sum_blocks * dim;
+  a.group = p.group;
+  a.groups = p.groups;
+  a.per_group = p.per_group;
+  if (grad_dtype == NR_DTYPE_F32) return launch_sum<float>(p, a, grad, st);
+  if (grad_dtype == NR_DTYPE_BF16) return launch_sum<__bf16>(p, a, grad, st);
+  return launch_sum<_Float16>(p, a, grad, st);
+}

@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(256)
 adam_kernel(float* __restrict__ param, float* __restrict__ grad, float* __restrict__ m, float* __restrict__ v,
             int64_t n, float lr, float beta1, float beta2, float eps, float wd, int adamw, float bc1, float bc2_sqrt,
             float grad_scale, int zero_grad, const float* __restrict__ dev_hyper, uint8_t* __restrict__ seen_grad,
-            const float* __restrict__ skip, __bf16* __restrict__ delta16, int ss) {
+            const float* __restrict__ skip, __bf16* __restrict__ delta16, int ss, const float* __restrict__ clip) {
   // ss: stride of the moments in 16-byte groups -- 1: two arrays; 2: ONE array of [exp_avg x4 | exp_avg_sq x4] records (v = m + 4
   // floats): a live group between never-touched neighbours then costs three cache lines (parameter, gradient, moments) instead of four
   if (skip != nullptr && skip[0] != 0.0f) {  // found-inf (GradScaler.step): no update; the gradient is still cleared
@@ -115,6 +115,7 @@ adam_kernel(float* __restrict__ param, float* __restrict__ grad, float* __restri
     bc1 = dev_hyper[1];
     bc2_sqrt = dev_hyper[2];
   }
+  if (clip != nullptr) grad_scale *= clip[0];  // gradients clipped to a global norm (nr_grad_norm's factor)
   const int64_t n4 = n / 4;
   float4* p4 = reinterpret_cast<float4*>(param);
   float4* g4 = reinterpret_cast<float4*>(grad);
@@ -972,10 +973,10 @@ extern "C" int nr_sh4_fwd(const float* dirs, int64_t n, float* out, nr_stream_t 
   return 0;
 }
 
-extern "C" int nr_adam_step(float* param, float* grad, float* m, float* v, int64_t n, float lr, float beta1,
-                            float beta2, float eps, float wd, int adamw, int step, float grad_scale, int zero_grad,
-                            const float* dev_hyper, uint8_t* seen_grad, const float* skip, void* delta16, int state_stride,
-                            nr_stream_t stream) {
+extern "C" int nr_adam_step_clipped(float* param, float* grad, float* m, float* v, int64_t n, float lr, float beta1,
+                                    float beta2, float eps, float wd, int adamw, int step, float grad_scale, int zero_grad,
+                                    const float* dev_hyper, uint8_t* seen_grad, const float* skip, void* delta16, int state_stride,
+                                    const float* clip, nr_stream_t stream) {
   if (n == 0) return 0;
   if (!param || !grad || !m || !v || n < 0 || step < 1) return NR_EINVAL;
   if (state_stride != 1 && !(state_stride == 2 && (n & 3) == 0 && v == m + 4)) return NR_EINVAL;
@@ -986,9 +987,18 @@ extern "C" int nr_adam_step(float* param, float* grad, float* m, float* v, int64
   const int64_t cap = nr_tuning().adam_blocks > 0 ? nr_tuning().adam_blocks : 4096;
   const unsigned blocks = (unsigned)(want < cap ? want : cap);
   hipLaunchKernelGGL(adam_kernel, dim3(blocks), dim3(256), 0, nr_s(stream), param, grad, m, v, n, lr, beta1, beta2, eps,
-                     wd, adamw, bc1, bc2_sqrt, grad_scale, zero_grad, dev_hyper, seen_grad, skip, static_cast<__bf16*>(delta16), state_stride);
+                     wd, adamw, bc1, bc2_sqrt, grad_scale, zero_grad, dev_hyper, seen_grad, skip, static_cast<__bf16*>(delta16), state_stride,
+                     clip);
   NR_LAUNCH_CHECK();
   return 0;
+}
+
+extern "C" int nr_adam_step(float* param, float* grad, float* m, float* v, int64_t n, float lr, float beta1,
+                            float beta2, float eps, float wd, int adamw, int step, float grad_scale, int zero_grad,
+                            const float* dev_hyper, uint8_t* seen_grad, const float* skip, void* delta16, int state_stride,
+                            nr_stream_t stream) {
+  return nr_adam_step_clipped(param, grad, m, v, n, lr, beta1, beta2, eps, wd, adamw, step, grad_scale, zero_grad, dev_hyper, seen_grad,
+                              skip, delta16, state_stride, nullptr, stream);
 }
 
 extern "C" int nr_apply_delta16(float* param, const void* delta16, int64_t n, int64_t lo, int64_t hi, nr_stream_t stream) {

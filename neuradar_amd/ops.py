@@ -4,11 +4,14 @@ Every function here launches hand-written gfx950 kernels on torch's current stre
 on a ROCm device.  torch is plumbing only (memory, streams, autograd bookkeeping).
 """
 import os
+from array import array
+from contextlib import nullcontext
 from ctypes import byref, c_void_p
 from typing import List, Optional, Sequence, Tuple
 
 import torch
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import NrField, NrFieldGrads, NrMlp, NrMlpGrads, check
@@ -696,6 +699,131 @@ def radar_loss(pred: Tensor, detections: Tensor, seg: Tensor, max_detections: in
     return _RadarLoss.apply(pred, detections, seg, assoc, loss_type, float(mult)), assoc
 
 
+# ------------------------------------------------------------------------------------------------ embedding rows
+_DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # NR_DTYPE_*
+_NO_GUARD = nullcontext()
+
+
+def _on_device_of(t: Tensor):
+    """The tensor's device as the current one for a launch (streams, workspaces): nothing to do where it is already."""
+    return _NO_GUARD if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.get_device())
+
+
+def _float_rows(t: Tensor, what: str) -> Tensor:
+    if not t.is_cuda:
+        raise RuntimeError(f"{what} must be a GPU tensor: neuradar_amd has no CPU path (the oracle is test-only)")
+    if t.dtype not in _DTYPE_CODES:
+        raise RuntimeError(f"{what} must be float32, bfloat16 or float16, not {t.dtype}")
+    if t.dim() != 2:
+        raise RuntimeError(f"{what} must be [rows, dim], not {tuple(t.shape)}")
+    return t
+
+
+def _row_index(idx: Tensor, device: int) -> Tensor:
+    if idx.dtype not in (torch.int64, torch.int32):
+        raise RuntimeError(f"indices must be int64 or int32, not {idx.dtype}")
+    if idx.get_device() != device:
+        raise RuntimeError("indices must be on the table's device")
+    return idx.contiguous()
+
+
+def _padding_row(padding_idx: Optional[int], rows: int) -> int:
+    """nn.Embedding's convention: negative counts from the end; -1 (none) for the ABI."""
+    if padding_idx is None:
+        return -1
+    if not -rows <= padding_idx < rows:
+        raise RuntimeError(f"padding_idx {padding_idx} is not a row of a table of {rows}")
+    return padding_idx % rows
+
+
+def _strided_rows(t: Tensor) -> Tuple[Tensor, int]:
+    """[n, dim] as (tensor, elements between rows) with neighbouring columns: a copy only where the columns are apart."""
+    if (t.shape[1] > 1 and t.stride(1) != 1) or t.stride(0) < 0:
+        t = t.contiguous()
+    return t, t.stride(0)
+
+
+def _embedding_rows(table: Tensor, idx: Tensor, scale: float) -> Tensor:
+    rows, dim = table.shape
+    out = torch.empty((*idx.shape, dim), device=table.device, dtype=table.dtype)
+    table, stride = _strided_rows(table)
+    with _on_device_of(table):
+        check(_lib.lib().nr_embedding_fwd(table.data_ptr(), _DTYPE_CODES[table.dtype], rows, dim, stride, idx.data_ptr(), idx.element_size(),
+                                          idx.numel(), scale, out.data_ptr(), dim, _stream()), "nr_embedding_fwd")
+    return out
+
+
+def embedding_grad(grad: Tensor, idx: Tensor, num_rows: int, scale: float = 1.0, padding_idx: Optional[int] = None,
+                   out: Optional[Tensor] = None, accumulate: bool = False, dtype: Optional[torch.dtype] = None) -> Tensor:
+    """Gradient of `embedding` for its table: [num_rows, dim] with scale * (sum of grad[i] over idx[i] == v) in row v, by sorted
+    indices -- no atomics, the same bits on every call.  grad [*idx.shape, dim] (rows may be apart), fp32 / bf16 / fp16; sums in
+    fp32, rounded once to the result's type (`dtype`; grad's own by default).
+    out: contiguous [num_rows, dim] that takes the result; accumulate: added to what `out` holds (rows that no index names are not
+    touched).  Indices equal to padding_idx or outside [0, num_rows) contribute nothing."""
+    dim = grad.shape[-1] if grad.dim() > 0 else -1
+    if grad.shape != (*idx.shape, dim):
+        raise RuntimeError(f"grad {tuple(grad.shape)} does not fit indices {tuple(idx.shape)}")
+    grad = _float_rows(grad.reshape(idx.numel(), dim) if grad.dim() != 2 else grad, "grad")
+    idx = _row_index(idx, grad.get_device())
+    padding = _padding_row(padding_idx, num_rows)
+    if accumulate and out is None:
+        raise RuntimeError("accumulate=True adds to `out`: give it")
+    if out is None:
+        if dtype is not None and dtype not in _DTYPE_CODES:
+            raise RuntimeError(f"dtype must be float32, bfloat16 or float16, not {dtype}")
+        out = torch.empty((num_rows, dim), device=grad.device, dtype=grad.dtype if dtype is None else dtype)
+    elif (_float_rows(out, "out").shape != (num_rows, dim) or not out.is_contiguous() or out.get_device() != grad.get_device()
+          or dtype not in (None, out.dtype)):
+        raise RuntimeError(f"out must be a contiguous [{num_rows}, {dim}] tensor on grad's device" + ("" if dtype is None else f" of {dtype}"))
+    grad, stride = _strided_rows(grad)
+    n, code = idx.numel(), _DTYPE_CODES[grad.dtype]
+    lib = _lib.lib()
+    need = lib.nr_embedding_bwd_workspace_bytes(num_rows, dim, n, code)
+    if need < 0:
+        raise RuntimeError(f"embedding_grad: sizes out of range ({n} indices, {num_rows} rows of {dim})")
+    with _on_device_of(grad):
+        workspace = torch.empty(need, device=grad.device, dtype=torch.uint8)
+        check(lib.nr_embedding_bwd(grad.data_ptr(), code, stride, idx.data_ptr(), idx.element_size(), n, num_rows, dim, scale, padding,
+                                   out.data_ptr(), _DTYPE_CODES[out.dtype], int(accumulate), workspace.data_ptr(), _stream()),
+              "nr_embedding_bwd")
+    return out
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, idx, scale, padding_idx):
+        ctx.save_for_backward(idx)
+        ctx.meta = (table.shape[0], table.dtype, scale, padding_idx)
+        ctx.table_ref = table
+        return _embedding_rows(table, idx, scale)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        (idx,) = ctx.saved_tensors
+        rows, dtype, scale, padding_idx = ctx.meta
+        table = ctx.table_ref
+        if (_DIRECT_PARAM_GRADS and table.is_leaf and table.requires_grad and table.grad is not None and table.grad.is_contiguous()
+                and table.grad.dtype in _DTYPE_CODES):
+            embedding_grad(grad, idx, rows, scale, padding_idx, out=table.grad, accumulate=True)
+            return None, None, None, None
+        return embedding_grad(grad, idx, rows, scale, padding_idx, dtype=dtype), None, None, None
+
+
+def embedding(table: Tensor, idx: Tensor, scale: float = 1.0, padding_idx: Optional[int] = None) -> Tensor:
+    """scale * table[idx]: rows of an embedding table [rows, dim] (fp32 / bf16 / fp16; rows may be apart, columns neighbours) for
+    indices of any shape (int64 / int32) -> [*idx.shape, dim] in the table's type, one rounding.  An index outside [0, rows) gives
+    a row of NaN and no gradient (nothing is read on the host, so nothing can be raised).
+    Differentiable in the table: embedding_grad, inside `direct_param_grads` straight into table.grad.  padding_idx as in
+    nn.Embedding: that row is looked up like any other and gets no gradient."""
+    _float_rows(table, "table")
+    idx = _row_index(idx, table.get_device())
+    _padding_row(padding_idx, table.shape[0])
+    if table.requires_grad and torch.is_grad_enabled():
+        return _Embedding.apply(table, idx, float(scale), padding_idx)
+    return _embedding_rows(table, idx, float(scale))
+
+
 class _AppearanceConcat(torch.autograd.Function):
     """nr_appearance_concat_fwd/bwd: [features | temporal appearance embedding] of every ray (neuradar.py:510-512,550-568)."""
 
@@ -1178,16 +1306,134 @@ def conv_transpose3(x: Tensor, weight: Tensor, bias: Optional[Tensor]) -> Tensor
     return y.view(P, 3 * H, 3 * W, weight.shape[1]).permute(0, 3, 1, 2)
 
 
+# ------------------------------------------------------------------------------------------------ gradient norm and clipping
+_NORM_TYPES = {2.0: 2, 1.0: 1, float("inf"): 0}
+
+
+class _GradList:
+    """Addresses, sizes and types of a list of dense tensors as the host arrays that nr_grad_norm / nr_grad_scale read."""
+
+    def __init__(self, tensors: Sequence[Tensor], what: str) -> None:
+        try:
+            self.dtypes = array("i", [_DTYPE_CODES[t.dtype] for t in tensors])
+        except KeyError:
+            raise RuntimeError(f"{what} must be float32, bfloat16 or float16") from None
+        devices = {t.get_device() for t in tensors}
+        if len(devices) > 1 or -1 in devices:
+            raise RuntimeError(f"{what} must be GPU tensors on one device: neuradar_amd has no CPU path (the oracle is test-only)")
+        # (memory order is all that counts: a dense tensor is taken as it lies, one with holes is copied)
+        self.tensors = [t if t.is_contiguous() else _dense(t) for t in tensors]
+        self.ptrs = array("q", [t.data_ptr() for t in self.tensors])
+        self.numel = array("q", [t.numel() for t in self.tensors])
+        self.count = len(self.tensors)
+
+    @property
+    def arrays(self):
+        return [a.buffer_info()[0] for a in (self.ptrs, self.numel, self.dtypes)]
+
+
+def _dense(t: Tensor) -> Tensor:
+    """`t` itself if its elements fill a stretch of memory in some order of its dimensions (a channels-last weight), else a copy."""
+    if t.layout != torch.strided:
+        raise RuntimeError("sparse gradients are not supported")
+    order = sorted(range(t.dim()), key=lambda d: -t.stride(d))
+    p = t.permute(order)
+    return p if p.is_contiguous() else t.contiguous()
+
+
+def _norm_and_factor(lst: _GradList, max_norm: float, norm_type: float, device) -> Tensor:
+    """[norm, clip factor] on the device."""
+    kind = _NORM_TYPES.get(float(norm_type))
+    if kind is None:
+        raise RuntimeError(f"norm_type must be 1, 2 or infinity, not {norm_type}")
+    if not max_norm >= 0.0:
+        raise RuntimeError(f"max_norm must not be negative or NaN: {max_norm}")
+    lib = _lib.lib()
+    ptrs, numel, dtypes = lst.arrays
+    need = lib.nr_grad_norm_workspace_bytes(numel, lst.count)
+    if need < 0:
+        raise RuntimeError("gradient list too long")
+    workspace = torch.empty(2 + need // 4, device=device, dtype=torch.float32)  # [norm, factor | partial results]
+    check(lib.nr_grad_norm(ptrs, numel, dtypes, lst.count, kind, max_norm, workspace.data_ptr(), workspace.data_ptr() + 8, _stream()),
+          "nr_grad_norm")
+    return workspace
+
+
+def _as_list(tensors) -> List[Tensor]:
+    return [tensors] if isinstance(tensors, Tensor) else list(tensors)
+
+
+def grad_norm(grads, norm_type: float = 2.0) -> Tensor:
+    """Global norm (norm_type 2, 1 or infinity) over all elements of a tensor or of a sequence of tensors (fp32 / bf16 / fp16, mixed)
+    -> fp32 scalar tensor.  Two launches for up to 96 tensors; nothing is read on the host; sums in fp64 in a fixed order."""
+    grads = _as_list(grads)
+    if not grads:
+        return torch.zeros((), device="cuda", dtype=torch.float32)
+    lst = _GradList(grads, "gradients")
+    with _on_device_of(grads[0]):
+        return _norm_and_factor(lst, float("inf"), norm_type, grads[0].device)[0]
+
+
+def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> Tensor:
+    """Scale gradients by min(1, max_norm / (norm + 1e-6)), norm = grad_norm(grads, norm_type), which is returned.  In place, or
+    into the tensors of `out` (same shapes, any of the three types: a 16-bit bucket, say), one rounding.  Nothing is read on
+    the host; a norm of NaN makes every gradient NaN, as in torch."""
+    grads = _as_list(grads)
+    targets = grads if out is None else _as_list(out)
+    if len(targets) != len(grads) or any(o.shape != g.shape for o, g in zip(targets, grads)):
+        raise RuntimeError("out must hold one tensor of the same shape for each gradient")
+    if not grads:
+        return torch.zeros((), device="cuda", dtype=torch.float32)
+    src = _GradList(grads, "gradients")
+    dst = src if out is None else _GradList(targets, "out")
+    if len({p for p, n in zip(dst.ptrs, dst.numel) if n}) != sum(1 for n in dst.numel if n):
+        raise RuntimeError("a tensor to be written is listed twice")
+    # a target with holes is written through its dense copy; source and target elements must lie in the same order
+    if out is not None and any(not o.is_contiguous() or not g.is_contiguous() for o, g in zip(targets, grads)):
+        src = _GradList([g.contiguous() for g in grads], "gradients")
+        dst = _GradList([o if o.is_contiguous() else torch.empty_like(o, memory_format=torch.contiguous_format) for o in targets], "out")
+    with _on_device_of(grads[0]):
+        result = _norm_and_factor(src, float(max_norm), norm_type, grads[0].device)
+        ptrs, numel, dtypes = src.arrays
+        check(_lib.lib().nr_grad_scale(ptrs, dst.arrays[0], numel, dtypes, dst.arrays[2], src.count, result.data_ptr(), _stream()),
+              "nr_grad_scale")
+        for target, written in zip(targets, dst.tensors):
+            if written.data_ptr() != target.data_ptr():
+                target.copy_(written)
+    return result[0]
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False) -> Tensor:
+    """torch.nn.utils.clip_grad_norm_ on the framework's kernels: clip the .grad of `parameters` (those that have one) to a global
+    norm, in place, and return the norm.  error_if_nonfinite reads it on the host (not inside a graph capture)."""
+    grads, seen = [], set()
+    for p in _as_list(parameters):
+        if p.grad is not None and id(p) not in seen:
+            seen.add(id(p))
+            grads.append(p.grad)
+    if not grads:
+        return torch.zeros((), dtype=torch.float32)
+    if error_if_nonfinite:
+        norm = grad_norm(grads, norm_type)
+        if not bool(torch.isfinite(norm)):
+            raise RuntimeError(f"the total norm of order {norm_type} of the gradients is not finite, so they cannot be clipped")
+    return clip_grads(grads, max_norm, norm_type)
+
+
 # ------------------------------------------------------------------------------------------------ optimizer
 def adam_step(param: Tensor, grad: Tensor, exp_avg: Tensor, exp_avg_sq: Tensor, lr: float, step: int,
               betas=(0.9, 0.999), eps: float = 1e-15, weight_decay: float = 0.0, adamw: bool = False,
               grad_scale: float = 1.0, zero_grad: bool = True, dev_hyper: Optional[Tensor] = None,
               seen_grad: Optional[Tensor] = None, marked: bool = False, skip: Optional[Tensor] = None,
-              delta16: Optional[Tensor] = None) -> None:
+              delta16: Optional[Tensor] = None, clip: Optional[Tensor] = None) -> None:
     """seen_grad: optional uint8 [numel/4], zero while exp_avg / exp_avg_sq are zero (see include/neuradar_hip.h).
     marked: the scatter sets the bytes (nr_hash_encode_bwd_marked) -- never-marked groups are skipped without reading their gradient.
     skip: optional device float (a loss scaler's found-inf flag): non-zero = no update, the gradient is still cleared (2.0: kept).
-    delta16: optional bf16 [numel]: the update leaves as a rounded delta that is also what the owner applies (sharded DP step)."""
+    delta16: optional bf16 [numel]: the update leaves as a rounded delta that is also what the owner applies (sharded DP step).
+    clip: optional device float that the gradient is multiplied by (the factor of a global norm), besides grad_scale."""
+    if clip is not None:
+        assert clip.dtype == torch.float32 and clip.is_cuda and not marked
     if delta16 is not None:
         assert delta16.dtype == torch.bfloat16 and delta16.numel() == param.numel() and delta16.is_contiguous() and not marked
     if seen_grad is not None:
@@ -1204,9 +1450,9 @@ def adam_step(param: Tensor, grad: Tensor, exp_avg: Tensor, exp_avg_sq: Tensor, 
                                              eps, step, grad_scale, int(zero_grad), _p(dev_hyper), _p(seen_grad), _p(skip), stride, _stream()),
               "nr_adam_step_marked")
         return
-    check(_lib.lib().nr_adam_step(_p(param), _p(grad), _p(exp_avg), _p(exp_avg_sq), param.numel(), lr, betas[0],
-                                  betas[1], eps, weight_decay, int(adamw), step, grad_scale, int(zero_grad),
-                                  _p(dev_hyper), _p(seen_grad), _p(skip), _p(delta16), stride, _stream()), "nr_adam_step")
+    check(_lib.lib().nr_adam_step_clipped(_p(param), _p(grad), _p(exp_avg), _p(exp_avg_sq), param.numel(), lr, betas[0],
+                                          betas[1], eps, weight_decay, int(adamw), step, grad_scale, int(zero_grad),
+                                          _p(dev_hyper), _p(seen_grad), _p(skip), _p(delta16), stride, _p(clip), _stream()), "nr_adam_step")
 
 
 def hash_mark_vertices(x: Tensor, scalings: Tensor, log2_hashmap_size: int, stamp: Tensor, epoch: Tensor) -> None:
