@@ -36,6 +36,7 @@ extern "C" int nr_init(void) {
   if (int rc = nr_init_conv7()) return rc;
   if (int rc = nr_init_encoder()) return rc;
   if (int rc = nr_init_radar()) return rc;
+  if (int rc = nr_init_embedding()) return rc;
   return 0;
 }
 

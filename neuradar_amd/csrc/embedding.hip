@@ -250,117 +250,171 @@ __device__ __forceinline__ void write_row(const SumArgs& a, uint32_t row, int co
 }
 
 constexpr int kMaxStretch = 4096;  // sorted positions of one block (32 KB of LDS)
-constexpr int kFlight = 8;  // rows of g requested before the first of them is added
+constexpr int kFlight = 8;         // rows of g requested before the first of them is added
+
+// One group's stretch [q0, q1) of sorted tokens, on its columns: sums that start and end inside are written; a first sum that
+// started before the stretch is left in `head`, a last one that goes on behind it in `tail`.  key_at(q): the key of token q, also
+// of the one before the stretch and the one behind it; pos_at(q): its row of g.  Returns kHead | kSpan | kTail.  (Keys and
+// positions of a batch are read before anything is written: the compiler cannot know that a result is not one of them.)
+template <typename T, int N, typename Key, typename Pos>
+__device__ __forceinline__ uint32_t walk_stretch(const SumArgs& a, const T* __restrict__ grad, int q0, int q1, int col, uint32_t row0, Key key_at,
+                                                 Pos pos_at, float* head, float* tail) {
+  uint32_t flag = 0u;
+  float acc[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) acc[k] = 0.0f;
+  uint32_t key[kFlight + 1];
+  key[kFlight] = key_at(q0);
+  bool open_here = key_at(q0 - 1) != key[kFlight];
+  for (int q = q0; q < q1; q += kFlight) {
+    float x[kFlight][N];
+    uint32_t pos[kFlight];
+    key[0] = key[kFlight];
+#pragma unroll
+    for (int u = 0; u < kFlight; ++u) {
+      const bool in = q + u < q1;
+      pos[u] = in ? pos_at(q + u) : 0u;
+      key[u + 1] = in ? key_at(q + u + 1) : 0u;
+    }
+#pragma unroll
+    for (int u = 0; u < kFlight; ++u)
+      if (q + u < q1) nr_load_some<T, N>(grad + (int64_t)pos[u] * a.grad_stride + col, a.dim - col, x[u]);
+#pragma unroll
+    for (int u = 0; u < kFlight; ++u) {
+      if (q + u >= q1) break;
+      const bool goes_on = key[u] == key[u + 1];
+#pragma unroll
+      for (int k = 0; k < N; ++k) acc[k] += x[u][k];
+      if (goes_on && q + u + 1 < q1) continue;
+      float* part = nullptr;
+      if (!open_here) {
+        part = head;
+        flag |= goes_on ? kHead | kSpan : kHead;
+      } else if (goes_on) {
+        part = tail;
+        flag |= kTail;
+      }
+      if (part != nullptr) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) part[k] = acc[k];
+      } else {
+        write_row<N>(a, row0 + key[u], col, acc);
+      }
+      open_here = true;
+#pragma unroll
+      for (int k = 0; k < N; ++k) acc[k] = 0.0f;
+    }
+  }
+  return flag;
+}
+
+// Which groups hand a sum on whole, one bit each (call with all threads, between barriers of the caller's).
+__device__ __forceinline__ void mark_spans(const unsigned char* flags, int groups, uint64_t* span) {
+  const int g = threadIdx.x;
+  const uint64_t bits = __ballot(g < groups && (flags[g < groups ? g : 0] & kSpan) != 0u);
+  if (nr_lane() == 0) span[g / NR_WAVE] = bits;
+}
+
+// acc += the heads of groups j, j + 1, ... up to the first that does not hand its sum on; in order, kFlight requested at a time.
+// Returns whether there is such a group (the sum ended among them).
+template <int N>
+__device__ __forceinline__ bool follow_heads(const uint64_t* span, int j, int groups, const float* head, int step, float (&acc)[N]) {
+  int end = groups;  // the first group from j on without the bit
+  for (int w = j / NR_WAVE; w * NR_WAVE < groups; ++w) {
+    const uint64_t stops = ~span[w] & (w == j / NR_WAVE ? ~0ull << (j % NR_WAVE) : ~0ull);
+    if (stops != 0ull) {
+      end = w * NR_WAVE + __ffsll((unsigned long long)stops) - 1;
+      break;
+    }
+  }
+  const bool ended = end < groups;
+  const float* p = head + j * step;
+  int left = (ended ? end + 1 : groups) - j;
+  for (; left > 0; left -= kFlight, p += kFlight * step) {
+    float x[kFlight][N];
+#pragma unroll
+    for (int u = 0; u < kFlight; ++u)
+#pragma unroll
+      for (int k = 0; k < N; ++k) x[u][k] = u < left ? p[u * step + k] : 0.0f;
+#pragma unroll
+    for (int u = 0; u < kFlight; ++u)
+#pragma unroll
+      for (int k = 0; k < N; ++k) acc[k] += x[u][k];
+  }
+  return ended;
+}
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 sum_kernel(SumArgs a, const T* __restrict__ grad) {
   constexpr int N = 16 / (int)sizeof(T);
   extern __shared__ uint32_t lds[];
-  const int per_block = a.groups * a.per_group;
-  uint32_t* s_key = lds;                            // [per_block + 2]: the keys before, in and behind the stretch
+  const int per_block = a.groups * a.per_group, step = a.group * N;
+  float* s_head = reinterpret_cast<float*>(lds);    // [groups][group * N]
+  float* s_tail = s_head + a.groups * step;
+  uint32_t* s_key = reinterpret_cast<uint32_t*>(s_tail + a.groups * step);  // [per_block + 2]: the keys before, in and behind the stretch
   uint32_t* s_pos = s_key + per_block + 2;          // [per_block]
-  uint32_t* s_flag = s_pos + per_block;             // [groups]
-  uint32_t* s_left = s_flag + a.groups;             // [groups]: what a group leaves for the blocks around this one
-  float* s_head = reinterpret_cast<float*>(s_left + a.groups);  // [groups][group * N]
-  float* s_tail = s_head + a.groups * a.group * N;
+  unsigned char* s_flag = reinterpret_cast<unsigned char*>(s_pos + per_block);  // [groups]
+  unsigned char* s_left = s_flag + a.groups;        // [groups]: what a group leaves for the blocks around this one
+  __shared__ int s_valid;
+  __shared__ uint64_t s_span[kThreads / NR_WAVE];
   const int64_t p0 = (int64_t)blockIdx.x * per_block;
   constexpr uint32_t kNone = 0xFFFFFFFFu;
+  const uint32_t ignored = (uint32_t)a.rows;
+  if (threadIdx.x == 0) s_valid = 0;
+  __syncthreads();
+  int valid = 0;
   for (int i = threadIdx.x; i < per_block + 2; i += kThreads) {
     const int64_t p = p0 + i - 1;
-    s_key[i] = (p >= 0 && p < a.n) ? a.keys[p] : kNone;
-    if (i >= 1 && i <= per_block) s_pos[i - 1] = p < a.n ? a.pos[p] : 0u;
+    const uint32_t key = (p >= 0 && p < a.n) ? a.keys[p] : kNone;
+    s_key[i] = key;
+    if (i >= 1 && i <= per_block) {
+      s_pos[i - 1] = p < a.n ? a.pos[p] : 0u;
+      if (key < ignored) valid = i;
+    }
   }
+  if (valid > 0) atomicMax(&s_valid, valid);  // (keys ascend: what gets no gradient is behind everything else)
   __syncthreads();
+  const int count = s_valid;
   const int r = threadIdx.x / a.group, lane = threadIdx.x - r * a.group;
   const int col = (blockIdx.y * a.group + lane) * N;
   const bool work = r < a.groups && col < a.dim;
-  const uint32_t ignored = (uint32_t)a.rows;
-  float acc[N];
+  float* head = s_head + r * step + lane * N;
+  float* tail = s_tail + r * step + lane * N;
   if (work) {
-    const int q0 = r * a.per_group;
+    const int q0 = r * a.per_group, q1 = q0 + a.per_group < count ? q0 + a.per_group : count;
     uint32_t flag = 0u;
-    bool open_here = s_key[q0] != s_key[q0 + 1];  // does the first sum start in this stretch?
-#pragma unroll
-    for (int k = 0; k < N; ++k) acc[k] = 0.0f;
-    for (int q = q0; q < q0 + a.per_group; q += kFlight) {
-      float x[kFlight][N];
-#pragma unroll
-      for (int u = 0; u < kFlight; ++u) {
-        if (q + u < q0 + a.per_group && s_key[q + u + 1] < ignored) {
-          nr_load_some<T, N>(grad + (int64_t)s_pos[q + u] * a.grad_stride + col, a.dim - col, x[u]);
-        } else {
-#pragma unroll
-          for (int k = 0; k < N; ++k) x[u][k] = 0.0f;
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < kFlight; ++u) {
-        const int at = q + u;
-        if (at >= q0 + a.per_group) break;
-        const uint32_t key = s_key[at + 1], next = s_key[at + 2];
-        if (key >= ignored) break;  // (padding, out of range, behind the end: nothing follows)
-#pragma unroll
-        for (int k = 0; k < N; ++k) acc[k] += x[u][k];
-        const bool last = at + 1 == q0 + a.per_group;
-        if (key != next || last) {
-          const bool goes_on = key == next;
-          float* part = nullptr;
-          if (!open_here) {
-            part = s_head + (r * a.group + lane) * N;
-            flag |= goes_on ? kHead | kSpan : kHead;
-          } else if (goes_on) {
-            part = s_tail + (r * a.group + lane) * N;
-            flag |= kTail;
-          }
-          if (part != nullptr) {
-#pragma unroll
-            for (int k = 0; k < N; ++k) part[k] = acc[k];
-          } else {
-            write_row<N>(a, key, col, acc);
-          }
-          open_here = true;
-#pragma unroll
-          for (int k = 0; k < N; ++k) acc[k] = 0.0f;
-        }
-      }
-    }
-    if (lane == 0) s_flag[r] = flag;
+    if (q0 < q1)
+      flag = walk_stretch<T, N>(a, grad, q0, q1, col, 0u, [&](int q) { return s_key[q + 1]; }, [&](int q) { return s_pos[q]; }, head, tail);
+    if (lane == 0) s_flag[r] = (unsigned char)flag;
   }
+  __syncthreads();
+  mark_spans(s_flag, a.groups, s_span);
   __syncthreads();
   // sums that cross stretches: their first group adds the parts behind it, in order.  Group 0 also takes a sum that came in
   // from the block before.
   if (work) {
     const uint32_t own = s_flag[r];
-    auto follow = [&](int j) {  // adds the heads of groups j, j + 1, ...; true: the sum ended in this block
-      for (; j < a.groups; ++j) {
-        const float* part = s_head + (j * a.group + lane) * N;
-#pragma unroll
-        for (int k = 0; k < N; ++k) acc[k] += part[k];
-        if ((s_flag[j] & kSpan) == 0u) return true;
-      }
-      return false;
-    };
+    float acc[N];
     uint32_t flag = 0u;
     const int64_t slot = (int64_t)blockIdx.x * a.dim + col;
     if (r == 0 && (own & kHead)) {
 #pragma unroll
       for (int k = 0; k < N; ++k) acc[k] = 0.0f;
-      flag |= follow(0) ? kHead : kHead | kSpan;
+      flag |= follow_heads<N>(s_span, 0, a.groups, s_head + lane * N, step, acc) ? kHead : kHead | kSpan;
       nr_store_some<float, N>(a.head + slot, a.dim - col, acc);
     }
     if (own & kTail) {
-      const float* part = s_tail + (r * a.group + lane) * N;
 #pragma unroll
-      for (int k = 0; k < N; ++k) acc[k] = part[k];
-      if (follow(r + 1)) {
+      for (int k = 0; k < N; ++k) acc[k] = tail[k];
+      if (follow_heads<N>(s_span, r + 1, a.groups, s_head + lane * N, step, acc)) {
         write_row<N>(a, s_key[(r + 1) * a.per_group], col, acc);
       } else {
         nr_store_some<float, N>(a.tail + slot, a.dim - col, acc);
         flag |= kTail;
       }
     }
-    if (blockIdx.y == 0 && lane == 0) s_left[r] = flag;
+    if (blockIdx.y == 0 && lane == 0) s_left[r] = (unsigned char)flag;
   }
   __syncthreads();
   if (blockIdx.y == 0 && threadIdx.x == 0) {
@@ -370,24 +424,254 @@ sum_kernel(SumArgs a, const T* __restrict__ grad) {
   }
 }
 
-// A sum that starts in block b and leaves it: tail[b] + head[b + 1] + ... + the head that ends it.  One thread per 4 columns,
-// blocks in order.
-__global__ void __launch_bounds__(kThreads)
+// -------------------------------------------------------------------------------------------------- few indices: one launch
+// Up to kOwnMax indices: no sort of the whole, no workspace.  A block OWNS a range of rows (and of columns): it reads all
+// indices, keeps those of its range in ascending position (one ballot per 64), orders that short list by row, and sums it as
+// above; the rows of its range that nothing looks up it clears itself.  The indices are read by every block (128 KB from L2 at
+// 16 384 of 8 bytes), which is what limits the method to few of them.  A list is as long as the range's share of the tokens:
+// 64 on average, all of them at worst -- then one block per column range does the work, which is why columns are split
+// down to 64 bytes where there are fewer rows than blocks to fill the chip with.
+constexpr int kOwnThreads = 1024;
+constexpr int kOwnRounds = 16;
+constexpr int kOwnMax = kOwnThreads * kOwnRounds;  // 14 bits of position, 18 of row in a list entry
+constexpr int kOwnPosBits = 14;
+constexpr int kOwnRangeMax = 1 << (32 - kOwnPosBits - 1);
+constexpr int kOwnBlocks = 256;
+constexpr int kCountSort = 256;  // lists up to this length: every entry counts the smaller ones
+constexpr int kOwnDigitBits = 8;
+
+struct OwnArgs {
+  SumArgs sum;
+  int64_t padding;
+  int range, key_bits;  // rows per block; bits of a row inside its range
+};
+
+template <typename T, typename I, int ROUNDS>
+__global__ void __launch_bounds__(kOwnThreads)
+own_kernel(OwnArgs o, const T* __restrict__ grad, const I* __restrict__ idx) {
+  constexpr int N = 16 / (int)sizeof(T), kWaves = kOwnThreads / NR_WAVE;
+  const SumArgs& a = o.sum;
+  extern __shared__ uint32_t lds[];
+  const int step = a.group * N, lane = nr_lane(), wave = threadIdx.x / NR_WAVE;
+  float* s_head = reinterpret_cast<float*>(lds);             // [groups][group * N]
+  float* s_tail = s_head + a.groups * step;
+  uint32_t* s_digit = lds;                                   // [waves][256]: before the sums
+  uint32_t* s_list = lds + 2 * kOwnThreads * N;              // [ROUNDS * kOwnThreads]
+  unsigned char* s_flag = reinterpret_cast<unsigned char*>(s_list + ROUNDS * kOwnThreads);  // [groups]
+  __shared__ uint32_t s_count[kWaves];
+  __shared__ uint64_t s_span[kWaves];
+  const int64_t row0 = (int64_t)blockIdx.x * o.range;
+  const int range = row0 + o.range < a.rows ? o.range : (int)(a.rows - row0);
+  const int r = threadIdx.x / a.group, glane = threadIdx.x - r * a.group;
+  const int col = (blockIdx.y * a.group + glane) * N;
+  const bool work = r < a.groups && col < a.dim;
+
+  uint32_t item[ROUNDS];
+  constexpr uint32_t kNone = 0xFFFFFFFFu;
+#pragma unroll
+  for (int u = 0; u < ROUNDS; ++u) {
+    const int i = wave * (NR_WAVE * ROUNDS) + u * NR_WAVE + lane;
+    item[u] = kNone;
+    if (i < a.n) {
+      const int64_t v = (int64_t)idx[i];
+      if (v >= row0 && v < row0 + range && v != o.padding) item[u] = ((uint32_t)(v - row0) << kOwnPosBits) | (uint32_t)i;
+    }
+  }
+  if (!a.accumulate && work) {  // all rows of the range; those that are looked up are written again below, behind the barriers
+    const float zero[N] = {};
+    for (int q = r; q < range; q += a.groups) {
+      const int64_t at = (row0 + q) * a.dim + col;
+      if (a.out_dtype == NR_DTYPE_F32) nr_store_some<float, N>(static_cast<float*>(a.out) + at, a.dim - col, zero);
+      else nr_store_some<__bf16, N>(static_cast<__bf16*>(a.out) + at, a.dim - col, zero);  // (zero is zero in both 16-bit types)
+    }
+  }
+  uint32_t mine = 0u;
+#pragma unroll
+  for (int u = 0; u < ROUNDS; ++u) mine += (uint32_t)__popcll(__ballot(item[u] != kNone));
+  if (lane == 0) s_count[wave] = mine;
+  __syncthreads();
+  uint32_t at = 0u, total = 0u;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    at += w < wave ? s_count[w] : 0u;
+    total += s_count[w];
+  }
+  const int m = (int)total;
+  if (m == 0) return;
+#pragma unroll
+  for (int u = 0; u < ROUNDS; ++u) {
+    const uint64_t hit = __ballot(item[u] != kNone);
+    if (item[u] != kNone) s_list[at + (uint32_t)__popcll(hit & ((1ull << lane) - 1ull))] = item[u];
+    at += (uint32_t)__popcll(hit);
+  }
+  __syncthreads();
+  if (range > 1 && m <= kCountSort) {
+    // the entries are all different and ordered like (row, position): an entry's place is the number of smaller ones
+    uint32_t own = 0u;
+    int place = 0;
+    if ((int)threadIdx.x < m) {
+      own = s_list[threadIdx.x];
+      for (int j = 0; j < m; ++j) place += s_list[j] < own ? 1 : 0;
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < m) s_list[place] = own;
+    __syncthreads();
+  } else if (range > 1) {
+    // by 8 bits of the row at a time, as in sort_scatter_kernel: the list through registers and back
+    for (int shift = 0; shift < o.key_bits; shift += kOwnDigitBits) {
+      constexpr int kDigits = 1 << kOwnDigitBits;
+      for (int d = threadIdx.x; d < kWaves * kDigits; d += kOwnThreads) s_digit[d] = 0u;
+      uint32_t rank[ROUNDS];
+#pragma unroll
+      for (int u = 0; u < ROUNDS; ++u) {
+        const int i = wave * (NR_WAVE * ROUNDS) + u * NR_WAVE + lane;
+        item[u] = i < m ? s_list[i] : kNone;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < ROUNDS; ++u) {
+        const bool in = item[u] != kNone;
+        const uint32_t d = (item[u] >> (kOwnPosBits + shift)) & (kDigits - 1);
+        uint64_t peers = __ballot(in);
+        rank[u] = 0u;
+        if (peers == 0ull) continue;
+#pragma unroll
+        for (int b = 0; b < kOwnDigitBits; ++b) {
+          const uint64_t ones = __ballot((d >> b) & 1u);
+          peers &= ((d >> b) & 1u) ? ones : ~ones;
+        }
+        const int leader = in ? __ffsll((unsigned long long)peers) - 1 : lane;
+        uint32_t old = 0u;
+        if (in && lane == leader) old = atomicAdd(&s_digit[wave * kDigits + d], (uint32_t)__popcll(peers));
+        old = __shfl(old, leader, NR_WAVE);
+        rank[u] = old + (uint32_t)__popcll(peers & ((1ull << lane) - 1ull));
+      }
+      __syncthreads();
+      // exclusive prefix over (digit, wave): a thread per digit adds its waves, the first wave scans the 256 sums
+      __shared__ uint32_t s_first[kDigits];
+      if (threadIdx.x < kDigits) {
+        uint32_t sum = 0u;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+          const uint32_t c = s_digit[w * kDigits + threadIdx.x];
+          s_digit[w * kDigits + threadIdx.x] = sum;
+          sum += c;
+        }
+        s_first[threadIdx.x] = sum;
+      }
+      __syncthreads();
+      if (wave == 0) {
+        uint32_t c[4], sum = 0u;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          c[k] = s_first[lane * 4 + k];
+          sum += c[k];
+        }
+        uint32_t incl = sum;
+#pragma unroll
+        for (int d = 1; d < NR_WAVE; d <<= 1) {
+          const uint32_t t = __shfl_up(incl, d, NR_WAVE);
+          if (lane >= d) incl += t;
+        }
+        uint32_t run = incl - sum;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          s_first[lane * 4 + k] = run;
+          run += c[k];
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < ROUNDS; ++u) {
+        if (item[u] == kNone) continue;
+        const uint32_t d = (item[u] >> (kOwnPosBits + shift)) & (kDigits - 1);
+        s_list[s_first[d] + s_digit[wave * kDigits + d] + rank[u]] = item[u];
+      }
+      __syncthreads();
+    }
+  }
+  // the sums: the groups share the list evenly, a batch of loads at least
+  const int share = (m + a.groups - 1) / a.groups, per = share > kFlight ? share : kFlight;
+  auto key_at = [&](int q) { return q >= 0 && q < m ? s_list[q] >> kOwnPosBits : kNone; };
+  float* head = s_head + r * step + glane * N;
+  float* tail = s_tail + r * step + glane * N;
+  const int q0 = r * per, q1 = q0 + per < m ? q0 + per : m;
+  if (work) {
+    uint32_t flag = 0u;
+    if (q0 < q1)
+      flag = walk_stretch<T, N>(a, grad, q0, q1, col, (uint32_t)row0, key_at,
+                                [&](int q) { return s_list[q] & ((1u << kOwnPosBits) - 1u); }, head, tail);
+    if (glane == 0) s_flag[r] = (unsigned char)flag;
+  }
+  __syncthreads();
+  mark_spans(s_flag, a.groups, s_span);
+  __syncthreads();
+  if (work && (s_flag[r] & kTail)) {
+    float acc[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) acc[k] = tail[k];
+    follow_heads<N>(s_span, r + 1, a.groups, s_head + glane * N, step, acc);
+    write_row<N>(a, (uint32_t)row0 + key_at(q1 - 1), col, acc);
+  }
+}
+
+// A sum that starts in block b and leaves it: tail[b] + head[b + 1] + ... + the head that ends it.  A row that thousands of
+// tokens share crosses hundreds of blocks: groups of threads add consecutive shares of them, then the shares are added in order.
+constexpr int kJoinThreads = 512;
+constexpr int kJoinGroups = 64;
+__global__ void __launch_bounds__(kJoinThreads)
 join_kernel(SumArgs a, uint32_t blocks) {
   const uint32_t b = blockIdx.x;
   if ((a.flags[b] & kTail) == 0u) return;
+  __shared__ uint32_t s_end;
+  __shared__ float s_part[kJoinThreads * 4];
+  if (threadIdx.x == 0) s_end = blocks;
+  __syncthreads();
+  for (uint32_t j0 = b + 1; j0 < blocks; j0 += kJoinThreads) {  // the first block from b + 1 on that ends the sum
+    const uint32_t j = j0 + threadIdx.x;
+    if (j < blocks && (a.flags[j] & kSpan) == 0u) atomicMin(&s_end, j);
+    __syncthreads();
+    const uint32_t end = s_end;
+    __syncthreads();
+    if (end < blocks) break;
+  }
+  const int heads = (int)(s_end - b);  // blocks b + 1 .. s_end
   const int64_t per_block = (int64_t)a.groups * a.per_group;
   const uint32_t key = a.keys[(b + 1) * per_block - 1];
-  for (int col = threadIdx.x * 4; col < a.dim; col += kThreads * 4) {
-    float acc[4], x[4];
-    nr_load_some<float, 4>(a.tail + (int64_t)b * a.dim + col, a.dim - col, acc);
-    for (uint32_t j = b + 1; j < blocks; ++j) {
-      nr_load_some<float, 4>(a.head + (int64_t)j * a.dim + col, a.dim - col, x);
+  const int nv = (a.dim + 3) / 4, lanes = nv < kJoinThreads ? nv : kJoinThreads;
+  int groups = kJoinThreads / lanes < kJoinGroups ? kJoinThreads / lanes : kJoinGroups;
+  if (groups > (heads + kFlight - 1) / kFlight) groups = (heads + kFlight - 1) / kFlight;
+  const int per = (heads + groups - 1) / groups;
+  const int r = threadIdx.x / lanes, lane = threadIdx.x - r * lanes;
+  for (int col0 = 0; col0 < a.dim; col0 += lanes * 4) {
+    const int col = col0 + lane * 4;
+    const bool work = r < groups && col < a.dim;
+    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (work) {
+      if (r == 0) nr_load_some<float, 4>(a.tail + (int64_t)b * a.dim + col, a.dim - col, acc);
+      const int h1 = (r + 1) * per < heads ? (r + 1) * per : heads;
+      for (int h = r * per; h < h1; h += kFlight) {
+        float x[kFlight][4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) acc[k] += x[k];
-      if ((a.flags[j] & kSpan) == 0u) break;
+        for (int u = 0; u < kFlight; ++u)
+          if (h + u < h1) nr_load_some<float, 4>(a.head + (int64_t)(b + 1 + h + u) * a.dim + col, a.dim - col, x[u]);
+#pragma unroll
+        for (int u = 0; u < kFlight; ++u)
+          if (h + u < h1)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[k] += x[u][k];
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s_part[(r * lanes + lane) * 4 + k] = acc[k];
     }
-    write_row<4>(a, key, col, acc);
+    __syncthreads();
+    if (work && r == 0) {
+      for (int g = 1; g < groups; ++g)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[k] += s_part[(g * lanes + lane) * 4 + k];
+      write_row<4>(a, key, col, acc);
+    }
+    __syncthreads();
   }
 }
 
@@ -441,6 +725,27 @@ Plan make_plan(int64_t rows, int dim, int64_t n, int elem_size) {
   return p;
 }
 
+// The one-launch method: how many columns and rows a block owns.
+struct OwnPlan {
+  int group, groups, col_tiles, range, ranges, key_bits;
+};
+OwnPlan make_own_plan(int64_t rows, int dim, int elem_size) {
+  OwnPlan p = {};
+  const int vec = 16 / elem_size, nv = (dim + vec - 1) / vec;
+  int lanes = nv < NR_WAVE ? nv : NR_WAVE;  // a kilobyte of a row, then down to 64 bytes while there are CUs without a block
+  while (lanes > 4 && rows * ((nv + lanes - 1) / lanes) < kOwnBlocks) lanes = (lanes + 1) / 2;
+  p.col_tiles = (nv + lanes - 1) / lanes;
+  p.group = (nv + p.col_tiles - 1) / p.col_tiles;
+  p.groups = kOwnThreads / p.group;
+  const int64_t want = p.col_tiles < kOwnBlocks ? (kOwnBlocks + p.col_tiles - 1) / p.col_tiles : 1;
+  int64_t range = (rows + want - 1) / want;
+  if (range > kOwnRangeMax) range = kOwnRangeMax;
+  p.range = (int)range;
+  p.ranges = (int)((rows + range - 1) / range);
+  while (((range - 1) >> p.key_bits) != 0) ++p.key_bits;
+  return p;
+}
+
 bool sizes_ok(int64_t rows, int dim, int64_t n) {
   return rows >= 0 && rows <= 0x7FFFFFFE && dim >= 0 && dim <= kMaxDim && n >= 0 && n <= 0x7FFFFFFF;
 }
@@ -484,15 +789,47 @@ template <typename T>
 int launch_sum(const Plan& p, const SumArgs& a, const void* grad, hipStream_t stream) {
   constexpr int N = 16 / (int)sizeof(T);
   const int per_block = a.groups * a.per_group;
-  const size_t lds = (size_t)(2 * per_block + 2 + 2 * a.groups + 2 * a.groups * a.group * N) * 4;
+  const size_t lds = (size_t)(2 * per_block + 2 + 2 * a.groups * a.group * N) * 4 + (size_t)(2 * a.groups);
   hipLaunchKernelGGL(sum_kernel<T>, dim3(p.sum_blocks, (uint32_t)p.col_tiles), dim3(kThreads), lds, stream, a, static_cast<const T*>(grad));
   NR_LAUNCH_CHECK();
-  hipLaunchKernelGGL(join_kernel, dim3(p.sum_blocks), dim3(kThreads), 0, stream, a, p.sum_blocks);
+  hipLaunchKernelGGL(join_kernel, dim3(p.sum_blocks), dim3(kJoinThreads), 0, stream, a, p.sum_blocks);
   NR_LAUNCH_CHECK();
   return 0;
 }
 
+constexpr size_t own_lds(int vec, int rounds) { return (size_t)(2 * kOwnThreads * vec + rounds * kOwnThreads) * 4 + kOwnThreads; }
+
+template <typename T, typename I>
+int launch_own(const OwnPlan& p, const OwnArgs& o, const void* grad, const void* idx, hipStream_t stream) {
+  constexpr int N = 16 / (int)sizeof(T);
+  const dim3 grid((uint32_t)p.ranges, (uint32_t)p.col_tiles), block(kOwnThreads);
+  const T* g = static_cast<const T*>(grad);
+  const I* x = static_cast<const I*>(idx);
+  if (o.sum.n <= 2 * kOwnThreads) hipLaunchKernelGGL((own_kernel<T, I, 2>), grid, block, own_lds(N, 2), stream, o, g, x);
+  else hipLaunchKernelGGL((own_kernel<T, I, kOwnRounds>), grid, block, own_lds(N, kOwnRounds), stream, o, g, x);
+  NR_LAUNCH_CHECK();
+  return 0;
+}
+
+template <typename T>
+int init_own() {
+  constexpr int N = 16 / (int)sizeof(T);
+  if (int rc = nr_raise_lds(own_kernel<T, int64_t, 2>, own_lds(N, 2))) return rc;
+  if (int rc = nr_raise_lds(own_kernel<T, int32_t, 2>, own_lds(N, 2))) return rc;
+  if (int rc = nr_raise_lds(own_kernel<T, int64_t, kOwnRounds>, own_lds(N, kOwnRounds))) return rc;
+  return nr_raise_lds(own_kernel<T, int32_t, kOwnRounds>, own_lds(N, kOwnRounds));
+}
+
+// Few indices go through the one-launch method; what it cannot hold in a list entry is sorted.
+bool owns(int64_t rows, int64_t n) { return n <= kOwnMax && rows <= (int64_t)kOwnRangeMax * kOwnBlocks; }
+
 }  // namespace
+
+int nr_init_embedding() {
+  if (int rc = init_own<float>()) return rc;
+  if (int rc = init_own<__bf16>()) return rc;
+  return init_own<_Float16>();
+}
 
 extern "C" int nr_embedding_fwd(const void* table, int dtype, int64_t rows, int dim, int64_t row_stride, const void* idx, int idx_bytes,
                                 int64_t n, float scale, void* out, int64_t out_stride, nr_stream_t stream) {
@@ -508,7 +845,7 @@ extern "C" int nr_embedding_fwd(const void* table, int dtype, int64_t rows, int 
 
 extern "C" int64_t nr_embedding_bwd_workspace_bytes(int64_t rows, int dim, int64_t n, int grad_dtype) {
   if (!dtype_ok(grad_dtype) || !sizes_ok(rows, dim, n)) return NR_EINVAL;
-  if (n == 0 || dim == 0 || rows == 0) return 0;
+  if (n == 0 || dim == 0 || rows == 0 || owns(rows, n)) return 0;
   return make_plan(rows, dim, n, dtype_size(grad_dtype)).bytes;
 }
 
@@ -519,8 +856,29 @@ extern "C" int nr_embedding_bwd(const void* grad, int grad_dtype, int64_t grad_s
     return NR_EINVAL;
   if (rows == 0 || dim == 0) return 0;
   if (grad_table == nullptr || (reinterpret_cast<uintptr_t>(grad_table) & (uintptr_t)(dtype_size(table_dtype) - 1)) != 0) return NR_EINVAL;
-  if (n > 0 && (grad == nullptr || idx == nullptr || workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0)) return NR_EINVAL;
+  if (n > 0 && (grad == nullptr || idx == nullptr)) return NR_EINVAL;
   hipStream_t st = nr_s(stream);
+  SumArgs a = {};
+  a.n = n;
+  a.rows = rows;
+  a.dim = dim;
+  a.grad_stride = grad_stride;
+  a.scale = scale;
+  a.out = grad_table;
+  a.out_dtype = table_dtype;
+  a.accumulate = accumulate;
+  if (n > 0 && owns(rows, n)) {
+    const OwnPlan p = make_own_plan(rows, dim, dtype_size(grad_dtype));
+    a.group = p.group;
+    a.groups = p.groups;
+    const OwnArgs o = {a, padding, p.range, p.key_bits};
+    if (idx_bytes == 8)
+      return grad_dtype == NR_DTYPE_F32 ? launch_own<float, int64_t>(p, o, grad, idx, st)
+             : grad_dtype == NR_DTYPE_BF16 ? launch_own<__bf16, int64_t>(p, o, grad, idx, st) : launch_own<_Float16, int64_t>(p, o, grad, idx, st);
+    return grad_dtype == NR_DTYPE_F32 ? launch_own<float, int32_t>(p, o, grad, idx, st)
+           : grad_dtype == NR_DTYPE_BF16 ? launch_own<__bf16, int32_t>(p, o, grad, idx, st) : launch_own<_Float16, int32_t>(p, o, grad, idx, st);
+  }
+  if (n > 0 && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0)) return NR_EINVAL;
   if (!accumulate) {
     // the whole table: rows that nothing looks up are zero
     const int64_t halves = rows * dim * (dtype_size(table_dtype) / 2);
@@ -542,17 +900,8 @@ extern "C" int nr_embedding_bwd(const void* grad, int grad_dtype, int64_t grad_s
   s.padding = padding;
   s.blocks = p.sort_blocks;
   if (int rc = idx_bytes == 8 ? launch_sort<int64_t>(p, s, idx, pairs, st) : launch_sort<int32_t>(p, s, idx, pairs, st)) return rc;
-  SumArgs a = {};
   a.keys = pairs[(p.passes - 1) % 2 * 2];
   a.pos = pairs[(p.passes - 1) % 2 * 2 + 1];
-  a.n = n;
-  a.rows = rows;
-  a.dim = dim;
-  a.grad_stride = grad_stride;
-  a.scale = scale;
-  a.out = grad_table;
-  a.out_dtype = table_dtype;
-  a.accumulate = accumulate;
   a.flags = reinterpret_cast<uint32_t*>(ws + p.off_flags);
   a.head = reinterpret_cast<float*>(ws + p.off_parts);
   a.tail = a.head + (int64_t)p.sum_blocks * dim;

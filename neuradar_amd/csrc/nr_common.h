@@ -44,6 +44,7 @@ __device__ __forceinline__ void nr_bump_generation(uint32_t* gen) {
 int nr_init_conv7();
 int nr_init_encoder();
 int nr_init_radar();
+int nr_init_embedding();
 template <typename Kern>
 inline int nr_raise_lds(Kern kern, size_t bytes) {
   return (int)hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);

@@ -5,7 +5,6 @@ on a ROCm device.  torch is plumbing only (memory, streams, autograd bookkeeping
 """
 import os
 from array import array
-from contextlib import nullcontext
 from ctypes import byref, c_void_p
 from typing import List, Optional, Sequence, Tuple
 
@@ -701,12 +700,13 @@ def radar_loss(pred: Tensor, detections: Tensor, seg: Tensor, max_detections: in
 
 # ------------------------------------------------------------------------------------------------ embedding rows
 _DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # NR_DTYPE_*
-_NO_GUARD = nullcontext()
+_raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream of a device as an address, without a Stream object
 
 
-def _on_device_of(t: Tensor):
-    """The tensor's device as the current one for a launch (streams, workspaces): nothing to do where it is already."""
-    return _NO_GUARD if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.get_device())
+def _launch_stream(device: int) -> int:
+    """The stream to launch on for tensors of `device`, which has to be the current device."""
+    _lib.ensure_device(device)
+    return _raw_stream(device)
 
 
 def _float_rows(t: Tensor, what: str) -> Tensor:
@@ -744,12 +744,15 @@ def _strided_rows(t: Tensor) -> Tuple[Tensor, int]:
 
 
 def _embedding_rows(table: Tensor, idx: Tensor, scale: float) -> Tensor:
+    device = table.get_device()
+    if device != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _embedding_rows(table, idx, scale)
     rows, dim = table.shape
-    out = torch.empty((*idx.shape, dim), device=table.device, dtype=table.dtype)
+    out = table.new_empty((*idx.shape, dim))
     table, stride = _strided_rows(table)
-    with _on_device_of(table):
-        check(_lib.lib().nr_embedding_fwd(table.data_ptr(), _DTYPE_CODES[table.dtype], rows, dim, stride, idx.data_ptr(), idx.element_size(),
-                                          idx.numel(), scale, out.data_ptr(), dim, _stream()), "nr_embedding_fwd")
+    check(_lib.lib().nr_embedding_fwd(table.data_ptr(), _DTYPE_CODES[table.dtype], rows, dim, stride, idx.data_ptr(), idx.element_size(),
+                                      idx.numel(), scale, out.data_ptr(), dim, _launch_stream(device)), "nr_embedding_fwd")
     return out
 
 
@@ -760,32 +763,35 @@ def embedding_grad(grad: Tensor, idx: Tensor, num_rows: int, scale: float = 1.0,
     fp32, rounded once to the result's type (`dtype`; grad's own by default).
     out: contiguous [num_rows, dim] that takes the result; accumulate: added to what `out` holds (rows that no index names are not
     touched).  Indices equal to padding_idx or outside [0, num_rows) contribute nothing."""
-    dim = grad.shape[-1] if grad.dim() > 0 else -1
-    if grad.shape != (*idx.shape, dim):
+    device = grad.get_device()
+    if device >= 0 and device != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return embedding_grad(grad, idx, num_rows, scale, padding_idx, out, accumulate, dtype)
+    if grad.dim() != idx.dim() + 1 or grad.shape[:-1] != idx.shape:
         raise RuntimeError(f"grad {tuple(grad.shape)} does not fit indices {tuple(idx.shape)}")
-    grad = _float_rows(grad.reshape(idx.numel(), dim) if grad.dim() != 2 else grad, "grad")
-    idx = _row_index(idx, grad.get_device())
+    n, dim = idx.numel(), grad.shape[-1]
+    grad = _float_rows(grad if grad.dim() == 2 else grad.reshape(n, dim), "grad")
+    idx = _row_index(idx, device)
     padding = _padding_row(padding_idx, num_rows)
-    if accumulate and out is None:
-        raise RuntimeError("accumulate=True adds to `out`: give it")
     if out is None:
+        if accumulate:
+            raise RuntimeError("accumulate=True adds to `out`: give it")
         if dtype is not None and dtype not in _DTYPE_CODES:
             raise RuntimeError(f"dtype must be float32, bfloat16 or float16, not {dtype}")
-        out = torch.empty((num_rows, dim), device=grad.device, dtype=grad.dtype if dtype is None else dtype)
-    elif (_float_rows(out, "out").shape != (num_rows, dim) or not out.is_contiguous() or out.get_device() != grad.get_device()
+        out = grad.new_empty((num_rows, dim), dtype=dtype)
+    elif (_float_rows(out, "out").shape != (num_rows, dim) or not out.is_contiguous() or out.get_device() != device
           or dtype not in (None, out.dtype)):
         raise RuntimeError(f"out must be a contiguous [{num_rows}, {dim}] tensor on grad's device" + ("" if dtype is None else f" of {dtype}"))
     grad, stride = _strided_rows(grad)
-    n, code = idx.numel(), _DTYPE_CODES[grad.dtype]
+    code = _DTYPE_CODES[grad.dtype]
     lib = _lib.lib()
     need = lib.nr_embedding_bwd_workspace_bytes(num_rows, dim, n, code)
     if need < 0:
         raise RuntimeError(f"embedding_grad: sizes out of range ({n} indices, {num_rows} rows of {dim})")
-    with _on_device_of(grad):
-        workspace = torch.empty(need, device=grad.device, dtype=torch.uint8)
-        check(lib.nr_embedding_bwd(grad.data_ptr(), code, stride, idx.data_ptr(), idx.element_size(), n, num_rows, dim, scale, padding,
-                                   out.data_ptr(), _DTYPE_CODES[out.dtype], int(accumulate), workspace.data_ptr(), _stream()),
-              "nr_embedding_bwd")
+    workspace = grad.new_empty(need, dtype=torch.uint8) if need else None
+    check(lib.nr_embedding_bwd(grad.data_ptr(), code, stride, idx.data_ptr(), idx.element_size(), n, num_rows, dim, scale, padding,
+                               out.data_ptr(), _DTYPE_CODES[out.dtype], accumulate, None if workspace is None else workspace.data_ptr(),
+                               _launch_stream(device)), "nr_embedding_bwd")
     return out
 
 
@@ -1314,28 +1320,31 @@ class _GradList:
     """Addresses, sizes and types of a list of dense tensors as the host arrays that nr_grad_norm / nr_grad_scale read."""
 
     def __init__(self, tensors: Sequence[Tensor], what: str) -> None:
-        try:
-            self.dtypes = array("i", [_DTYPE_CODES[t.dtype] for t in tensors])
-        except KeyError:
-            raise RuntimeError(f"{what} must be float32, bfloat16 or float16") from None
-        devices = {t.get_device() for t in tensors}
+        self.count = len(tensors)
+        dtypes = [t.dtype for t in tensors]
+        if not _DTYPE_CODES.keys() >= set(dtypes):
+            raise RuntimeError(f"{what} must be float32, bfloat16 or float16")
+        devices = set(map(Tensor.get_device, tensors))
         if len(devices) > 1 or -1 in devices:
             raise RuntimeError(f"{what} must be GPU tensors on one device: neuradar_amd has no CPU path (the oracle is test-only)")
         # (memory order is all that counts: a dense tensor is taken as it lies, one with holes is copied)
-        self.tensors = [t if t.is_contiguous() else _dense(t) for t in tensors]
-        self.ptrs = array("q", [t.data_ptr() for t in self.tensors])
-        self.numel = array("q", [t.numel() for t in self.tensors])
-        self.count = len(self.tensors)
+        self.plain = all(map(Tensor.is_contiguous, tensors))
+        self.tensors = tensors if self.plain else [_dense(t) for t in tensors]
+        self.ptrs = array("q", map(Tensor.data_ptr, self.tensors))
+        self.numel = array("q", map(Tensor.numel, self.tensors))
+        self.dtypes = array("i", map(_DTYPE_CODES.__getitem__, dtypes))
 
     @property
     def arrays(self):
-        return [a.buffer_info()[0] for a in (self.ptrs, self.numel, self.dtypes)]
+        return self.ptrs.buffer_info()[0], self.numel.buffer_info()[0], self.dtypes.buffer_info()[0]
 
 
 def _dense(t: Tensor) -> Tensor:
     """`t` itself if its elements fill a stretch of memory in some order of its dimensions (a channels-last weight), else a copy."""
     if t.layout != torch.strided:
         raise RuntimeError("sparse gradients are not supported")
+    if t.is_contiguous():
+        return t
     order = sorted(range(t.dim()), key=lambda d: -t.stride(d))
     p = t.permute(order)
     return p if p.is_contiguous() else t.contiguous()
@@ -1354,8 +1363,8 @@ def _norm_and_factor(lst: _GradList, max_norm: float, norm_type: float, device) 
     if need < 0:
         raise RuntimeError("gradient list too long")
     workspace = torch.empty(2 + need // 4, device=device, dtype=torch.float32)  # [norm, factor | partial results]
-    check(lib.nr_grad_norm(ptrs, numel, dtypes, lst.count, kind, max_norm, workspace.data_ptr(), workspace.data_ptr() + 8, _stream()),
-          "nr_grad_norm")
+    at = workspace.data_ptr()
+    check(lib.nr_grad_norm(ptrs, numel, dtypes, lst.count, kind, max_norm, at, at + 8, _launch_stream(device.index)), "nr_grad_norm")
     return workspace
 
 
@@ -1369,35 +1378,48 @@ def grad_norm(grads, norm_type: float = 2.0) -> Tensor:
     grads = _as_list(grads)
     if not grads:
         return torch.zeros((), device="cuda", dtype=torch.float32)
-    lst = _GradList(grads, "gradients")
-    with _on_device_of(grads[0]):
-        return _norm_and_factor(lst, float("inf"), norm_type, grads[0].device)[0]
+    device = grads[0].device
+    if device.type == "cuda" and device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return grad_norm(grads, norm_type)
+    return _norm_and_factor(_GradList(grads, "gradients"), float("inf"), norm_type, device)[0]
 
 
 def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> Tensor:
     """Scale gradients by min(1, max_norm / (norm + 1e-6)), norm = grad_norm(grads, norm_type), which is returned.  In place, or
-    into the tensors of `out` (same shapes, any of the three types: a 16-bit bucket, say), one rounding.  Nothing is read on
+    into the tensors of `out` (as many elements each, any of the three types: places in a 16-bit bucket, say), one rounding.  Nothing is read on
     the host; a norm of NaN makes every gradient NaN, as in torch."""
     grads = _as_list(grads)
     targets = grads if out is None else _as_list(out)
-    if len(targets) != len(grads) or any(o.shape != g.shape for o, g in zip(targets, grads)):
-        raise RuntimeError("out must hold one tensor of the same shape for each gradient")
+    if len(targets) != len(grads):
+        raise RuntimeError("out must hold one tensor of the same size for each gradient")
     if not grads:
         return torch.zeros((), device="cuda", dtype=torch.float32)
-    src = _GradList(grads, "gradients")
-    dst = src if out is None else _GradList(targets, "out")
-    if len({p for p, n in zip(dst.ptrs, dst.numel) if n}) != sum(1 for n in dst.numel if n):
+    device = grads[0].device
+    if device.type == "cuda" and device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return clip_grads(grads, max_norm, norm_type, out)
+    src = dst = _GradList(grads, "gradients")
+    if out is not None:
+        dst = _GradList(targets, "out")
+        if dst.numel != src.numel:
+            raise RuntimeError("out must hold one tensor of the same size for each gradient")
+        if not (src.plain and dst.plain):  # elements are matched by place in memory: bring both into the order of their shapes
+            if any(o.shape != g.shape for o, g in zip(targets, grads)):
+                raise RuntimeError("out must have its gradients' shapes where one of the two is not contiguous")
+            src = _GradList([g.contiguous() for g in grads], "gradients")
+            dst = _GradList([o if o.is_contiguous() else torch.empty_like(o, memory_format=torch.contiguous_format) for o in targets], "out")
+        if targets[0].device != device:
+            raise RuntimeError("out must be on the gradients' device")
+    filled = [p for p, n in zip(dst.ptrs, dst.numel) if n]
+    if len(set(filled)) != len(filled):
         raise RuntimeError("a tensor to be written is listed twice")
-    # a target with holes is written through its dense copy; source and target elements must lie in the same order
-    if out is not None and any(not o.is_contiguous() or not g.is_contiguous() for o, g in zip(targets, grads)):
-        src = _GradList([g.contiguous() for g in grads], "gradients")
-        dst = _GradList([o if o.is_contiguous() else torch.empty_like(o, memory_format=torch.contiguous_format) for o in targets], "out")
-    with _on_device_of(grads[0]):
-        result = _norm_and_factor(src, float(max_norm), norm_type, grads[0].device)
-        ptrs, numel, dtypes = src.arrays
-        check(_lib.lib().nr_grad_scale(ptrs, dst.arrays[0], numel, dtypes, dst.arrays[2], src.count, result.data_ptr(), _stream()),
-              "nr_grad_scale")
-        for target, written in zip(targets, dst.tensors):
+    result = _norm_and_factor(src, float(max_norm), norm_type, device)
+    ptrs, numel, dtypes = src.arrays
+    check(_lib.lib().nr_grad_scale(ptrs, dst.arrays[0], numel, dtypes, dst.arrays[2], src.count, result.data_ptr(),
+                                   _launch_stream(device.index)), "nr_grad_scale")
+    if not dst.plain or dst.tensors is not targets:
+        for target, written in zip(targets, dst.tensors):  # a target with holes gets its elements from a dense copy
             if written.data_ptr() != target.data_ptr():
                 target.copy_(written)
     return result[0]

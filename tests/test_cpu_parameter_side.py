@@ -16,7 +16,7 @@ def test_embedding_entry_points_refuse_bad_arguments():
     def fwd(table=BIG, dtype=0, rows=10, dim=8, stride=8, idx=BIG, idx_bytes=8, n=4, out=BIG, out_stride=8):
         return lib.nr_embedding_fwd(table, dtype, rows, dim, stride, idx, idx_bytes, n, 1.0, out, out_stride, None)
 
-    def bwd(grad=BIG, dtype=0, stride=8, idx=BIG, idx_bytes=8, n=4, rows=10, dim=8, out=BIG, out_dtype=0, workspace=BIG):
+    def bwd(grad=BIG, dtype=0, stride=8, idx=BIG, idx_bytes=8, n=20000, rows=10, dim=8, out=BIG, out_dtype=0, workspace=BIG):
         return lib.nr_embedding_bwd(grad, dtype, stride, idx, idx_bytes, n, rows, dim, 1.0, -1, out, out_dtype, 1, workspace, None)
 
     for kw in (dict(dtype=3), dict(dtype=-1), dict(rows=-1), dict(rows=0x7FFFFFFF), dict(dim=-1), dict(dim=65537), dict(idx_bytes=2), dict(n=-1),
@@ -30,7 +30,7 @@ def test_embedding_entry_points_refuse_bad_arguments():
         assert bwd(**kw) == E, kw
     assert bwd(rows=0) == 0 and bwd(dim=0) == 0 and bwd(n=0) == 0
     assert lib.nr_embedding_bwd_workspace_bytes(10, 8, -1, 0) == E and lib.nr_embedding_bwd_workspace_bytes(10, 8, 4, 5) == E
-    assert lib.nr_embedding_bwd_workspace_bytes(10, 8, 0, 0) == 0 and lib.nr_embedding_bwd_workspace_bytes(10, 8, 4, 0) > 0
+    assert lib.nr_embedding_bwd_workspace_bytes(10, 8, 0, 0) == 0 and lib.nr_embedding_bwd_workspace_bytes(10, 8, 20000, 0) > 0
 
 
 def test_norm_entry_points_refuse_bad_arguments():

@@ -160,9 +160,10 @@ def test_refusals():
     g = torch.ones(6, device=DEV)
     for call, what in ((lambda: ops.grad_norm([g], 3.0), "norm_type"), (lambda: ops.clip_grads([g], -1.0), "max_norm"),
                        (lambda: ops.clip_grads([g], float("nan")), "max_norm"), (lambda: ops.clip_grads([g, g], 1.0), "listed twice"),
-                       (lambda: ops.clip_grads([g, g + 1], 1.0, out=[g, g]), "listed twice"), (lambda: ops.clip_grads([g], 1.0, out=[g[:5]]), "same shape"),
-                       (lambda: ops.clip_grads([g], 1.0, out=[g, g]), "same shape"), (lambda: ops.clip_grads([g], 1.0, out=[g.double()]), "float32"),
-                       (lambda: ops.grad_norm([g, torch.ones(2)]), "one device"), (lambda: ops.grad_norm([g.to_sparse()]), "")):
+                       (lambda: ops.clip_grads([g, g + 1], 1.0, out=[g, g]), "listed twice"), (lambda: ops.clip_grads([g], 1.0, out=[g[:5]]), "same size"),
+                       (lambda: ops.clip_grads([g], 1.0, out=[g, g + 1]), "same size"), (lambda: ops.clip_grads([g], 1.0, out=[g.double()]), "float32"),
+                       (lambda: ops.grad_norm([g, torch.ones(2)]), "one device"), (lambda: ops.grad_norm([g.to_sparse()]), "."),
+                       (lambda: ops.clip_grads([g.view(2, 3).t()], 1.0, out=[g.clone()]), "shapes")):
         with pytest.raises(RuntimeError, match=what):
             call()
     assert bool((g == 1).all())
