@@ -21,7 +21,7 @@ namespace {
 
 constexpr int kMaxDim = 65536;
 constexpr int kThreads = 256;
-constexpr int kRounds = 8;                            // rounds of 64 tokens that a wave ranks in one tile of the sort
+constexpr int kRounds = 4;                            // rounds of 64 tokens that a wave ranks in one tile of the sort
 constexpr int kTile = kThreads * kRounds;             // tokens per block of the sort
 constexpr int kMaxDigitBits = 11;
 
@@ -67,13 +67,23 @@ rows_kernel(const T* __restrict__ table, int64_t rows, int dim, int64_t row_stri
   }
 }
 
+// thread t of `threads`: its share of `halves` 16-bit zeros at p
+__device__ __forceinline__ void clear_halves(uint16_t* __restrict__ p, int64_t halves, int64_t t, int64_t threads) {
+  typedef NrPack<uint16_t, 8> Pack;
+  Pack* q = reinterpret_cast<Pack*>(p);
+  const int64_t packs = halves / 8;
+  for (int64_t i = t; i < packs; i += threads) q[i].v = (Pack::vec)(uint16_t)0;
+  const int64_t rest = packs * 8 + t;
+  if (rest < halves) p[rest] = 0;
+}
+
 // ---------------------------------------------------------------------------------------------------------------- sort
 struct SortPass {
   const uint32_t* keys;   // NULL: this pass reads the indices themselves
   const uint32_t* pos;
   uint32_t* keys_out;
   uint32_t* pos_out;
-  uint32_t* counts;       // [digits][blocks]
+  uint32_t* counts;       // [blocks][digits]
   uint32_t* totals;       // [digits]
   int64_t n, rows, padding;
   int shift, bits;
@@ -92,63 +102,62 @@ __global__ void __launch_bounds__(kThreads)
 sort_count_kernel(SortPass s, const I* __restrict__ idx) {
   __shared__ uint32_t cnt[1 << kMaxDigitBits];
   const int digits = 1 << s.bits;
-  for (int d = threadIdx.x; d < digits; d += kThreads) cnt[d] = 0u;
-  __syncthreads();
   const int64_t base = (int64_t)blockIdx.x * kTile;
+  uint32_t key[kRounds];
 #pragma unroll
   for (int u = 0; u < kRounds; ++u) {
     const int64_t i = base + u * kThreads + threadIdx.x;
-    if (i < s.n) atomicAdd(&cnt[(key_of(s, idx, i) >> s.shift) & (uint32_t)(digits - 1)], 1u);
+    key[u] = i < s.n ? key_of(s, idx, i) : 0u;
   }
+  for (int d = threadIdx.x; d < digits; d += kThreads) cnt[d] = 0u;
   __syncthreads();
-  for (int d = threadIdx.x; d < digits; d += kThreads) s.counts[(int64_t)d * s.blocks + blockIdx.x] = cnt[d];
+#pragma unroll
+  for (int u = 0; u < kRounds; ++u)
+    if (base + u * kThreads + threadIdx.x < s.n) atomicAdd(&cnt[(key[u] >> s.shift) & (uint32_t)(digits - 1)], 1u);
+  __syncthreads();
+  for (int d = threadIdx.x; d < digits; d += kThreads) s.counts[(int64_t)blockIdx.x * digits + d] = cnt[d];
 }
 
-// counts[d][b] -> tokens of digit d in blocks before b; totals[d].  One wave per digit.
+// counts[b][d] -> tokens of digit d in blocks before b; totals[d].  A wave takes 16 digits and a quarter of the blocks for each
+// (lanes of one quarter read neighbouring digits), the quarters are then shifted by what lies before them.
+constexpr int kScanDigits = 16;
 __global__ void __launch_bounds__(kThreads)
 sort_scan_kernel(SortPass s) {
-  const int d = (int)(blockIdx.x * (kThreads / NR_WAVE) + threadIdx.x / NR_WAVE);
-  if (d >= (1 << s.bits)) return;
-  const int lane = nr_lane();
-  uint32_t* c = s.counts + (int64_t)d * s.blocks;
-  uint32_t before = 0u;
-  for (uint32_t b0 = 0; b0 < s.blocks; b0 += NR_WAVE) {
-    const uint32_t b = b0 + lane;
-    const uint32_t own = b < s.blocks ? c[b] : 0u;
-    uint32_t incl = own;
-#pragma unroll
-    for (int o = 1; o < NR_WAVE; o <<= 1) {
-      const uint32_t t = __shfl_up(incl, o, NR_WAVE);
-      if (lane >= o) incl += t;
-    }
-    if (b < s.blocks) c[b] = before + incl - own;
-    before += __shfl(incl, NR_WAVE - 1, NR_WAVE);
-  }
-  if (lane == 0) s.totals[d] = before;
-}
-
-// Exclusive prefix sums of x[0 .. count) in LDS by the whole block; scratch: kThreads words.
-__device__ __forceinline__ void block_exclusive_scan(uint32_t* x, int count, uint32_t* scratch) {
-  const int per = (count + kThreads - 1) / kThreads, lo = threadIdx.x * per;
+  constexpr int kParts = kThreads / kScanDigits;  // parts of the blocks
+  __shared__ uint32_t part[kParts][kScanDigits];
+  const int digits = 1 << s.bits;
+  const int d = blockIdx.x * kScanDigits + threadIdx.x % kScanDigits, q = threadIdx.x / kScanDigits;
+  const uint32_t per = (s.blocks + kParts - 1) / kParts, b0 = q * per, b1 = b0 + per < s.blocks ? b0 + per : s.blocks;
   uint32_t sum = 0u;
-  for (int k = 0; k < per; ++k)
-    if (lo + k < count) sum += x[lo + k];
-  scratch[threadIdx.x] = sum;
-  __syncthreads();
-  for (int o = 1; o < kThreads; o <<= 1) {
-    const uint32_t t = (int)threadIdx.x >= o ? scratch[threadIdx.x - o] : 0u;
-    __syncthreads();
-    scratch[threadIdx.x] += t;
-    __syncthreads();
-  }
-  uint32_t run = scratch[threadIdx.x] - sum;
-  for (int k = 0; k < per; ++k)
-    if (lo + k < count) {
-      const uint32_t own = x[lo + k];
-      x[lo + k] = run;
-      run += own;
+  if (d < digits)
+    for (uint32_t b = b0; b < b1; b += 4) {
+      uint32_t c[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) c[u] = b + u < b1 ? s.counts[(int64_t)(b + u) * digits + d] : 0u;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) sum += c[u];
     }
+  part[q][threadIdx.x % kScanDigits] = sum;
   __syncthreads();
+  uint32_t before = 0u, total = 0u;
+#pragma unroll
+  for (int k = 0; k < kParts; ++k) {
+    const uint32_t c = part[k][threadIdx.x % kScanDigits];
+    before += k < q ? c : 0u;
+    total += c;
+  }
+  if (d >= digits) return;
+  for (uint32_t b = b0; b < b1; b += 4) {
+    uint32_t c[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) c[u] = b + u < b1 ? s.counts[(int64_t)(b + u) * digits + d] : 0u;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (b + u < b1) s.counts[(int64_t)(b + u) * digits + d] = before;
+      before += c[u];
+    }
+  }
+  if (q == 0) s.totals[d] = total;
 }
 
 // A wave ranks 64 tokens at a time: lanes of equal digit find each other by one ballot per bit, the lowest of them advances the
@@ -156,19 +165,12 @@ __device__ __forceinline__ void block_exclusive_scan(uint32_t* x, int count, uin
 template <typename I>
 __global__ void __launch_bounds__(kThreads)
 sort_scatter_kernel(SortPass s, const I* __restrict__ idx) {
-  constexpr int kWaves = kThreads / NR_WAVE;
+  constexpr int kWaves = kThreads / NR_WAVE, kPer = (1 << kMaxDigitBits) / kThreads;  // digits per thread at most
   __shared__ uint32_t cnt[kWaves][1 << kMaxDigitBits];
-  __shared__ uint32_t first[1 << kMaxDigitBits];
-  __shared__ uint32_t scratch[kThreads];
+  __shared__ uint32_t s_wave[kWaves];
   const int digits = 1 << s.bits, lane = nr_lane(), wave = threadIdx.x / NR_WAVE;
-  for (int d = threadIdx.x; d < digits; d += kThreads) {
-    first[d] = s.totals[d];
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) cnt[w][d] = 0u;
-  }
-  __syncthreads();
   const int64_t base = (int64_t)blockIdx.x * kTile + (int64_t)wave * (NR_WAVE * kRounds);
-  uint32_t key[kRounds], pos[kRounds], rank[kRounds];
+  uint32_t key[kRounds], pos[kRounds], rank[kRounds], total[kPer], before[kPer];
 #pragma unroll
   for (int u = 0; u < kRounds; ++u) {
     const int64_t i = base + u * NR_WAVE + lane;
@@ -176,6 +178,16 @@ sort_scatter_kernel(SortPass s, const I* __restrict__ idx) {
     key[u] = in ? key_of(s, idx, i) : 0u;
     pos[u] = in ? (s.pos != nullptr ? s.pos[i] : (uint32_t)i) : 0u;
   }
+  // (thread t: digits t * per ... + per of the tables of counts)
+  const int per = digits > kThreads ? digits / kThreads : 1;
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    const int d = threadIdx.x * per + k;
+    const bool in = k < per && d < digits;
+    total[k] = in ? s.totals[d] : 0u;
+    before[k] = in ? s.counts[(int64_t)blockIdx.x * digits + d] : 0u;
+  }
+  for (int d = lane; d < digits; d += NR_WAVE) cnt[wave][d] = 0u;  // (a wave counts in its own row only: no barrier)
 #pragma unroll
   for (int u = 0; u < kRounds; ++u) {
     const bool in = base + u * NR_WAVE + lane < s.n;
@@ -191,16 +203,34 @@ sort_scatter_kernel(SortPass s, const I* __restrict__ idx) {
     old = __shfl(old, leader, NR_WAVE);
     rank[u] = old + (uint32_t)__popcll(peers & ((1ull << lane) - 1ull));
   }
-  __syncthreads();
-  block_exclusive_scan(first, digits, scratch);
-  for (int d = threadIdx.x; d < digits; d += kThreads) {
-    uint32_t at = first[d] + s.counts[(int64_t)d * s.blocks + blockIdx.x];
+  // first place of each digit: exclusive prefix of the totals over the threads, then over a thread's own digits
+  uint32_t sum = 0u;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const uint32_t own = cnt[w][d];
-      cnt[w][d] = at;
-      at += own;
+  for (int k = 0; k < kPer; ++k) sum += total[k];
+  uint32_t incl = sum;
+#pragma unroll
+  for (int o = 1; o < NR_WAVE; o <<= 1) {
+    const uint32_t t = __shfl_up(incl, o, NR_WAVE);
+    if (lane >= o) incl += t;
+  }
+  if (lane == NR_WAVE - 1) s_wave[wave] = incl;
+  __syncthreads();
+  uint32_t first = incl - sum;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) first += w < wave ? s_wave[w] : 0u;
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    const int d = threadIdx.x * per + k;
+    if (k < per && d < digits) {
+      uint32_t at = first + before[k];
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const uint32_t own = cnt[w][d];
+        cnt[w][d] = at;
+        at += own;
+      }
     }
+    first += total[k];
   }
   __syncthreads();
 #pragma unroll
@@ -477,12 +507,17 @@ own_kernel(OwnArgs o, const T* __restrict__ grad, const I* __restrict__ idx) {
       if (v >= row0 && v < row0 + range && v != o.padding) item[u] = ((uint32_t)(v - row0) << kOwnPosBits) | (uint32_t)i;
     }
   }
-  if (!a.accumulate && work) {  // all rows of the range; those that are looked up are written again below, behind the barriers
-    const float zero[N] = {};
-    for (int q = r; q < range; q += a.groups) {
-      const int64_t at = (row0 + q) * a.dim + col;
-      if (a.out_dtype == NR_DTYPE_F32) nr_store_some<float, N>(static_cast<float*>(a.out) + at, a.dim - col, zero);
-      else nr_store_some<__bf16, N>(static_cast<__bf16*>(a.out) + at, a.dim - col, zero);  // (zero is zero in both 16-bit types)
+  if (!a.accumulate) {  // all rows of the range; those that are looked up are written again below, behind the barriers
+    if (gridDim.y == 1) {
+      const int words = a.out_dtype == NR_DTYPE_F32 ? 2 : 1;
+      clear_halves(static_cast<uint16_t*>(a.out) + row0 * a.dim * words, (int64_t)range * a.dim * words, threadIdx.x, kOwnThreads);
+    } else if (work) {
+      const float zero[N] = {};
+      for (int q = r; q < range; q += a.groups) {
+        const int64_t at = (row0 + q) * a.dim + col;
+        if (a.out_dtype == NR_DTYPE_F32) nr_store_some<float, N>(static_cast<float*>(a.out) + at, a.dim - col, zero);
+        else nr_store_some<__bf16, N>(static_cast<__bf16*>(a.out) + at, a.dim - col, zero);  // (zero is zero in both 16-bit types)
+      }
     }
   }
   uint32_t mine = 0u;
@@ -677,12 +712,7 @@ join_kernel(SumArgs a, uint32_t blocks) {
 
 __global__ void __launch_bounds__(kThreads)
 clear_kernel(uint16_t* __restrict__ p, int64_t halves) {
-  typedef NrPack<uint16_t, 8> Pack;
-  const int64_t packs = halves / 8;
-  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < packs; i += (int64_t)gridDim.x * kThreads)
-    reinterpret_cast<Pack*>(p)[i].v = (Pack::vec)(uint16_t)0;
-  if (blockIdx.x == 0)
-    for (int64_t i = packs * 8 + threadIdx.x; i < halves; i += kThreads) p[i] = 0;
+  clear_halves(p, halves, (int64_t)blockIdx.x * kThreads + threadIdx.x, (int64_t)gridDim.x * kThreads);
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host
@@ -778,7 +808,7 @@ int launch_sort(const Plan& p, SortPass s, const void* idx, uint32_t* const (&pa
     s.keys_out = pairs[pass % 2 * 2];
     s.pos_out = pairs[pass % 2 * 2 + 1];
     hipLaunchKernelGGL(sort_count_kernel<I>, dim3(p.sort_blocks), dim3(kThreads), 0, stream, s, static_cast<const I*>(idx));
-    hipLaunchKernelGGL(sort_scan_kernel, dim3((uint32_t)nr_cdiv(1 << s.bits, kThreads / NR_WAVE)), dim3(kThreads), 0, stream, s);
+    hipLaunchKernelGGL(sort_scan_kernel, dim3((uint32_t)nr_cdiv(1 << s.bits, kScanDigits)), dim3(kThreads), 0, stream, s);
     hipLaunchKernelGGL(sort_scatter_kernel<I>, dim3(p.sort_blocks), dim3(kThreads), 0, stream, s, static_cast<const I*>(idx));
     NR_LAUNCH_CHECK();
   }

@@ -17,6 +17,7 @@ constexpr int kThreads = 256;
 constexpr int kList = 96;                    // tensors of one launch (kernel arguments: 3 KB of the 4 KB there are)
 constexpr int kVec = 8;                      // elements per access
 constexpr int kStep = kThreads * kVec;       // elements a block takes at a time
+constexpr int kUnroll = 4;                   // accesses in flight
 constexpr int64_t kMaxBlocks = 4096;         // pieces that a list is cut into, about
 
 enum { kNormMax = 0, kNormSum = 1, kNormTwo = 2 };
@@ -91,7 +92,17 @@ __device__ __forceinline__ double block_reduce(Acc<KIND> acc) {
 
 template <int KIND, typename T>
 __device__ __forceinline__ void piece_norm(Acc<KIND>& acc, const T* __restrict__ x, int64_t lo, int64_t hi) {
-  for (int64_t i = lo + threadIdx.x * kVec; i < hi; i += kStep) {
+  int64_t i = lo + threadIdx.x * kVec;
+  for (; i + (kUnroll - 1) * kStep + kVec <= hi; i += kUnroll * kStep) {
+    float v[kUnroll][kVec];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) nr_load_pack<T, kVec>(x + i + u * kStep, v[u]);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+      for (int k = 0; k < kVec; ++k) acc.take(v[u][k]);
+  }
+  for (; i < hi; i += kStep) {
     float v[kVec];
     nr_load_some<T, kVec>(x + i, hi - i < kVec ? (int)(hi - i) : kVec, v);
 #pragma unroll
@@ -118,7 +129,13 @@ template <int KIND>
 __global__ void __launch_bounds__(kThreads)
 norm_finish_kernel(const double* __restrict__ partial, int64_t count, double max_norm, float* __restrict__ result) {
   Acc<KIND> acc;
-  for (int64_t i = threadIdx.x; i < count; i += kThreads) acc.join(partial[i]);
+  for (int64_t i = threadIdx.x; i < count; i += 4 * kThreads) {
+    double v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) v[u] = i + u * kThreads < count ? partial[i + u * kThreads] : 0.0;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) acc.join(v[u]);
+  }
   double v = block_reduce<KIND>(acc);
   if (threadIdx.x == 0) {
     if constexpr (KIND == kNormTwo) v = sqrt(v);
@@ -130,7 +147,19 @@ norm_finish_kernel(const double* __restrict__ partial, int64_t count, double max
 
 template <typename T, typename O>
 __device__ __forceinline__ void piece_scale(const T* __restrict__ x, O* __restrict__ y, int64_t lo, int64_t hi, float f) {
-  for (int64_t i = lo + threadIdx.x * kVec; i < hi; i += kStep) {
+  int64_t i = lo + threadIdx.x * kVec;
+  for (; i + (kUnroll - 1) * kStep + kVec <= hi; i += kUnroll * kStep) {
+    float v[kUnroll][kVec];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) nr_load_pack<T, kVec>(x + i + u * kStep, v[u]);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+#pragma unroll
+      for (int k = 0; k < kVec; ++k) v[u][k] *= f;
+      nr_store_pack<O, kVec>(y + i + u * kStep, v[u]);
+    }
+  }
+  for (; i < hi; i += kStep) {
     const int m = hi - i < kVec ? (int)(hi - i) : kVec;
     float v[kVec];
     nr_load_some<T, kVec>(x + i, m, v);
@@ -149,9 +178,11 @@ __device__ __forceinline__ void piece_scale_to(const T* x, void* y, int out_dtyp
 __global__ void __launch_bounds__(kThreads)
 scale_kernel(List l, const float* __restrict__ result) {
   const float f = result[1];
-  const int t = tensor_of(l, blockIdx.x);
+  // backwards: what the norm read last is what the cache still holds
+  const uint32_t block = gridDim.x - 1 - blockIdx.x;
+  const int t = tensor_of(l, block);
   if (f == 1.0f && l.in[t] == l.out[t]) return;  // in place and within the norm: nothing to do
-  const int64_t lo = (int64_t)(blockIdx.x - l.first[t]) * l.piece;
+  const int64_t lo = (int64_t)(block - l.first[t]) * l.piece;
   const int64_t hi = lo + l.piece < l.numel[t] ? lo + l.piece : l.numel[t];
   if (l.in_dtype[t] == NR_DTYPE_F32) piece_scale_to(static_cast<const float*>(l.in[t]), l.out[t], l.out_dtype[t], lo, hi, f);
   else if (l.in_dtype[t] == NR_DTYPE_BF16) piece_scale_to(static_cast<const __bf16*>(l.in[t]), l.out[t], l.out_dtype[t], lo, hi, f);
