@@ -72,7 +72,11 @@ __device__ __forceinline__ void clear_halves(uint16_t* __restrict__ p, int64_t h
   typedef NrPack<uint16_t, 8> Pack;
   Pack* q = reinterpret_cast<Pack*>(p);
   const int64_t packs = halves / 8;
-  for (int64_t i = t; i < packs; i += threads) q[i].v = (Pack::vec)(uint16_t)0;
+  int64_t i = t;
+  for (; i + 3 * threads < packs; i += 4 * threads)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) q[i + u * threads].v = (Pack::vec)(uint16_t)0;
+  for (; i < packs; i += threads) q[i].v = (Pack::vec)(uint16_t)0;
   const int64_t rest = packs * 8 + t;
   if (rest < halves) p[rest] = 0;
 }

@@ -15,10 +15,10 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kList = 96;                    // tensors of one launch (kernel arguments: 3 KB of the 4 KB there are)
-constexpr int kVec = 8;                      // elements per access
-constexpr int kStep = kThreads * kVec;       // elements a block takes at a time
-constexpr int kUnroll = 4;                   // accesses in flight
-constexpr int64_t kMaxBlocks = 4096;         // pieces that a list is cut into, about
+constexpr int kUnroll = 4;                   // 16-byte accesses in flight per thread
+constexpr int kPiece = kThreads * kUnroll * 8;  // elements: pieces of whole batches for 16-bit and 32-bit types
+constexpr int64_t kMaxBlocks = 16384;        // pieces that a list is cut into, about
+constexpr int kFinishThreads = 1024;
 
 enum { kNormMax = 0, kNormSum = 1, kNormTwo = 2 };
 
@@ -29,7 +29,7 @@ struct List {
   uint32_t first[kList + 1];  // first block of each tensor
   uint8_t in_dtype[kList], out_dtype[kList];
   int count;
-  int64_t piece;              // elements per block, a multiple of kStep
+  int64_t piece;              // elements per block, a multiple of kPiece
 };
 
 __device__ __forceinline__ int tensor_of(const List& l, uint32_t block) {
@@ -70,9 +70,9 @@ __device__ __forceinline__ double shfl_down_f64(double v, int d) {
 }
 
 // over the block, in thread 0
-template <int KIND>
+template <int KIND, int THREADS>
 __device__ __forceinline__ double block_reduce(Acc<KIND> acc) {
-  __shared__ double part[kThreads / NR_WAVE];
+  __shared__ double part[THREADS / NR_WAVE];
   if constexpr (KIND == kNormMax) acc.v = (double)__uint_as_float(acc.bits);
 #pragma unroll
   for (int d = NR_WAVE / 2; d > 0; d >>= 1) {
@@ -84,29 +84,31 @@ __device__ __forceinline__ double block_reduce(Acc<KIND> acc) {
   __syncthreads();
   if (threadIdx.x == 0) {
 #pragma unroll
-    for (int w = 1; w < kThreads / NR_WAVE; ++w) acc.join(part[w]);
+    for (int w = 1; w < THREADS / NR_WAVE; ++w) acc.join(part[w]);
     if constexpr (KIND == kNormMax) acc.v = (double)__uint_as_float(acc.bits);
   }
   return acc.v;
 }
 
+// Elements [lo, hi) of x: a lane takes 16 bytes, a wave a kilobyte, a block four such stretches in flight.
 template <int KIND, typename T>
 __device__ __forceinline__ void piece_norm(Acc<KIND>& acc, const T* __restrict__ x, int64_t lo, int64_t hi) {
-  int64_t i = lo + threadIdx.x * kVec;
-  for (; i + (kUnroll - 1) * kStep + kVec <= hi; i += kUnroll * kStep) {
-    float v[kUnroll][kVec];
+  constexpr int N = 16 / (int)sizeof(T), kStep = kThreads * N;
+  int64_t i = lo + threadIdx.x * N;
+  for (; i + (kUnroll - 1) * kStep + N <= hi; i += kUnroll * kStep) {
+    float v[kUnroll][N];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) nr_load_pack<T, kVec>(x + i + u * kStep, v[u]);
+    for (int u = 0; u < kUnroll; ++u) nr_load_pack<T, N>(x + i + u * kStep, v[u]);
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
 #pragma unroll
-      for (int k = 0; k < kVec; ++k) acc.take(v[u][k]);
+      for (int k = 0; k < N; ++k) acc.take(v[u][k]);
   }
   for (; i < hi; i += kStep) {
-    float v[kVec];
-    nr_load_some<T, kVec>(x + i, hi - i < kVec ? (int)(hi - i) : kVec, v);
+    float v[N];
+    nr_load_some<T, N>(x + i, hi - i < N ? (int)(hi - i) : N, v);
 #pragma unroll
-    for (int k = 0; k < kVec; ++k) acc.take(v[k]);
+    for (int k = 0; k < N; ++k) acc.take(v[k]);
   }
 }
 
@@ -120,23 +122,23 @@ norm_kernel(List l, double* __restrict__ partial) {
   if (l.in_dtype[t] == NR_DTYPE_F32) piece_norm<KIND, float>(acc, static_cast<const float*>(l.in[t]), lo, hi);
   else if (l.in_dtype[t] == NR_DTYPE_BF16) piece_norm<KIND, __bf16>(acc, static_cast<const __bf16*>(l.in[t]), lo, hi);
   else piece_norm<KIND, _Float16>(acc, static_cast<const _Float16*>(l.in[t]), lo, hi);
-  const double v = block_reduce<KIND>(acc);
+  const double v = block_reduce<KIND, kThreads>(acc);
   if (threadIdx.x == 0) partial[blockIdx.x] = v;
 }
 
 // result[0] = norm, result[1] = the factor that clips to max_norm
 template <int KIND>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kFinishThreads)
 norm_finish_kernel(const double* __restrict__ partial, int64_t count, double max_norm, float* __restrict__ result) {
   Acc<KIND> acc;
-  for (int64_t i = threadIdx.x; i < count; i += 4 * kThreads) {
+  for (int64_t i = threadIdx.x; i < count; i += 4 * kFinishThreads) {
     double v[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) v[u] = i + u * kThreads < count ? partial[i + u * kThreads] : 0.0;
+    for (int u = 0; u < 4; ++u) v[u] = i + u * kFinishThreads < count ? partial[i + u * kFinishThreads] : 0.0;
 #pragma unroll
     for (int u = 0; u < 4; ++u) acc.join(v[u]);
   }
-  double v = block_reduce<KIND>(acc);
+  double v = block_reduce<KIND, kFinishThreads>(acc);
   if (threadIdx.x == 0) {
     if constexpr (KIND == kNormTwo) v = sqrt(v);
     const double f = max_norm / (v + 1e-6);
@@ -147,25 +149,26 @@ norm_finish_kernel(const double* __restrict__ partial, int64_t count, double max
 
 template <typename T, typename O>
 __device__ __forceinline__ void piece_scale(const T* __restrict__ x, O* __restrict__ y, int64_t lo, int64_t hi, float f) {
-  int64_t i = lo + threadIdx.x * kVec;
-  for (; i + (kUnroll - 1) * kStep + kVec <= hi; i += kUnroll * kStep) {
-    float v[kUnroll][kVec];
+  constexpr int N = 16 / (int)sizeof(T), kStep = kThreads * N;
+  int64_t i = lo + threadIdx.x * N;
+  for (; i + (kUnroll - 1) * kStep + N <= hi; i += kUnroll * kStep) {
+    float v[kUnroll][N];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) nr_load_pack<T, kVec>(x + i + u * kStep, v[u]);
+    for (int u = 0; u < kUnroll; ++u) nr_load_pack<T, N>(x + i + u * kStep, v[u]);
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
 #pragma unroll
-      for (int k = 0; k < kVec; ++k) v[u][k] *= f;
-      nr_store_pack<O, kVec>(y + i + u * kStep, v[u]);
+      for (int k = 0; k < N; ++k) v[u][k] *= f;
+      nr_store_pack<O, N>(y + i + u * kStep, v[u]);
     }
   }
   for (; i < hi; i += kStep) {
-    const int m = hi - i < kVec ? (int)(hi - i) : kVec;
-    float v[kVec];
-    nr_load_some<T, kVec>(x + i, m, v);
+    const int m = hi - i < N ? (int)(hi - i) : N;
+    float v[N];
+    nr_load_some<T, N>(x + i, m, v);
 #pragma unroll
-    for (int k = 0; k < kVec; ++k) v[k] *= f;
-    nr_store_some<O, kVec>(y + i, m, v);
+    for (int k = 0; k < N; ++k) v[k] *= f;
+    nr_store_some<O, N>(y + i, m, v);
   }
 }
 template <typename T>
@@ -203,7 +206,7 @@ bool cut_list(const int64_t* numel, int count, Cut* c) {
     if (numel[t] < 0 || numel[t] > ((int64_t)1 << 40)) return false;
     total += numel[t];
   }
-  c->piece = nr_cdiv(total > 0 ? total : 1, kMaxBlocks * kStep) * kStep;
+  c->piece = nr_cdiv(total > 0 ? total : 1, kMaxBlocks * kPiece) * kPiece;
   c->blocks = 0;
   for (int t = 0; t < count; ++t) c->blocks += nr_cdiv(numel[t], c->piece);
   return c->blocks <= 0x7FFFFFFF;
@@ -258,7 +261,7 @@ int run_norm(const void* const* in, const int64_t* numel, const int32_t* dtype, 
     return 0;
   });
   if (rc != 0) return rc;
-  hipLaunchKernelGGL(norm_finish_kernel<KIND>, dim3(1), dim3(kThreads), 0, stream, partial, c.blocks, max_norm, result);
+  hipLaunchKernelGGL(norm_finish_kernel<KIND>, dim3(1), dim3(kFinishThreads), 0, stream, partial, c.blocks, max_norm, result);
   NR_LAUNCH_CHECK();
   return 0;
 }
