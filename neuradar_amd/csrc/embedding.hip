@@ -24,13 +24,14 @@ constexpr int kThreads = 256;
 constexpr int kRounds = 4;                            // rounds of 64 tokens that a wave ranks in one tile of the sort
 constexpr int kTile = kThreads * kRounds;             // tokens per block of the sort
 constexpr int kMaxDigitBits = 11;
+constexpr int64_t kZeroBlocks = 2048;                 // blocks of a launch that write zeros
 
 // ---------------------------------------------------------------------------------------------------------------- rows
 constexpr int kRowUnroll = 4;
 
 // Flat over the 16-byte vectors of the output, four per thread: every lane has work whatever the width is.  A row's last vector
 // may be short (dim not a multiple of the vector): element by element.
-template <typename T, typename I>
+template <typename T, typename I, bool STREAM>
 __global__ void __launch_bounds__(kThreads)
 rows_kernel(const T* __restrict__ table, int64_t rows, int dim, int64_t row_stride, const I* __restrict__ idx, int64_t n, float scale,
             T* __restrict__ out, int64_t out_stride, uint32_t nv, uint32_t magic) {
@@ -63,7 +64,9 @@ rows_kernel(const T* __restrict__ table, int64_t rows, int dim, int64_t row_stri
     if (r[u] >= n) continue;
 #pragma unroll
     for (int k = 0; k < N; ++k) x[u][k] *= scale;
-    nr_store_some<T, N>(out + r[u] * out_stride + col[u], dim - col[u], x[u]);
+    T* o = out + r[u] * out_stride + col[u];
+    if (STREAM && dim - col[u] >= N) nr_store_pack_stream<T, N>(o, x[u]);
+    else nr_store_some<T, N>(o, dim - col[u], x[u]);
   }
 }
 
@@ -77,8 +80,7 @@ __device__ __forceinline__ void clear_halves(uint16_t* __restrict__ p, int64_t h
 #pragma unroll
     for (int u = 0; u < 4; ++u) q[i + u * threads].v = (Pack::vec)(uint16_t)0;
   for (; i < packs; i += threads) q[i].v = (Pack::vec)(uint16_t)0;
-  const int64_t rest = packs * 8 + t;
-  if (rest < halves) p[rest] = 0;
+  for (int64_t rest = packs * 8 + t; rest < halves; rest += threads) p[rest] = 0;
 }
 
 // ---------------------------------------------------------------------------------------------------------------- sort
@@ -92,7 +94,19 @@ struct SortPass {
   int64_t n, rows, padding;
   int shift, bits;
   uint32_t blocks;
+  // the result's zeros: a share of them with each launch of the sort, in blocks behind its own -- the sort waits for memory more
+  // than it uses it (131 072 x 512 bf16: 21 us as a launch of its own)
+  uint16_t* zeros;
+  int64_t halves;
+  uint32_t zero_blocks;
 };
+
+// Whether this block is one of those behind `blocks`, and its work is done.
+__device__ __forceinline__ bool clears(const SortPass& s, uint32_t blocks) {
+  if (blockIdx.x < blocks) return false;
+  clear_halves(s.zeros, s.halves, (int64_t)(blockIdx.x - blocks) * kThreads + threadIdx.x, (int64_t)s.zero_blocks * kThreads);
+  return true;
+}
 
 template <typename I>
 __device__ __forceinline__ uint32_t key_of(const SortPass& s, const I* __restrict__ idx, int64_t i) {
@@ -105,6 +119,7 @@ template <typename I>
 __global__ void __launch_bounds__(kThreads)
 sort_count_kernel(SortPass s, const I* __restrict__ idx) {
   __shared__ uint32_t cnt[1 << kMaxDigitBits];
+  if (clears(s, s.blocks)) return;
   const int digits = 1 << s.bits;
   const int64_t base = (int64_t)blockIdx.x * kTile;
   uint32_t key[kRounds];
@@ -130,6 +145,7 @@ sort_scan_kernel(SortPass s) {
   constexpr int kParts = kThreads / kScanDigits;  // parts of the blocks
   __shared__ uint32_t part[kParts][kScanDigits];
   const int digits = 1 << s.bits;
+  if (clears(s, (uint32_t)(digits + kScanDigits - 1) / kScanDigits)) return;
   const int d = blockIdx.x * kScanDigits + threadIdx.x % kScanDigits, q = threadIdx.x / kScanDigits;
   const uint32_t per = (s.blocks + kParts - 1) / kParts, b0 = q * per, b1 = b0 + per < s.blocks ? b0 + per : s.blocks;
   uint32_t sum = 0u;
@@ -172,6 +188,7 @@ sort_scatter_kernel(SortPass s, const I* __restrict__ idx) {
   constexpr int kWaves = kThreads / NR_WAVE, kPer = (1 << kMaxDigitBits) / kThreads;  // digits per thread at most
   __shared__ uint32_t cnt[kWaves][1 << kMaxDigitBits];
   __shared__ uint32_t s_wave[kWaves];
+  if (clears(s, s.blocks)) return;
   const int digits = 1 << s.bits, lane = nr_lane(), wave = threadIdx.x / NR_WAVE;
   const int64_t base = (int64_t)blockIdx.x * kTile + (int64_t)wave * (NR_WAVE * kRounds);
   uint32_t key[kRounds], pos[kRounds], rank[kRounds], total[kPer], before[kPer];
@@ -478,6 +495,7 @@ struct OwnArgs {
   SumArgs sum;
   int64_t padding;
   int range, key_bits;  // rows per block; bits of a row inside its range
+  int list_words;       // n, rounded up
 };
 
 template <typename T, typename I, int ROUNDS>
@@ -490,8 +508,8 @@ own_kernel(OwnArgs o, const T* __restrict__ grad, const I* __restrict__ idx) {
   float* s_head = reinterpret_cast<float*>(lds);             // [groups][group * N]
   float* s_tail = s_head + a.groups * step;
   uint32_t* s_digit = lds;                                   // [waves][256]: before the sums
-  uint32_t* s_list = lds + 2 * kOwnThreads * N;              // [ROUNDS * kOwnThreads]
-  unsigned char* s_flag = reinterpret_cast<unsigned char*>(s_list + ROUNDS * kOwnThreads);  // [groups]
+  uint32_t* s_list = lds + 2 * kOwnThreads * N;              // [list_words]
+  unsigned char* s_flag = reinterpret_cast<unsigned char*>(s_list + o.list_words);  // [groups]
   __shared__ uint32_t s_count[kWaves];
   __shared__ uint64_t s_span[kWaves];
   const int64_t row0 = (int64_t)blockIdx.x * o.range;
@@ -661,6 +679,9 @@ constexpr int kJoinGroups = 64;
 __global__ void __launch_bounds__(kJoinThreads)
 join_kernel(SumArgs a, uint32_t blocks) {
   const uint32_t b = blockIdx.x;
+  const uint32_t near = b + 1 + threadIdx.x < blocks ? a.flags[b + 1 + threadIdx.x] : kSpan;
+  const int64_t per_block = (int64_t)a.groups * a.per_group;
+  const uint32_t key = a.keys[(b + 1) * per_block < a.n ? (b + 1) * per_block - 1 : a.n - 1];
   if ((a.flags[b] & kTail) == 0u) return;
   __shared__ uint32_t s_end;
   __shared__ float s_part[kJoinThreads * 4];
@@ -668,15 +689,13 @@ join_kernel(SumArgs a, uint32_t blocks) {
   __syncthreads();
   for (uint32_t j0 = b + 1; j0 < blocks; j0 += kJoinThreads) {  // the first block from b + 1 on that ends the sum
     const uint32_t j = j0 + threadIdx.x;
-    if (j < blocks && (a.flags[j] & kSpan) == 0u) atomicMin(&s_end, j);
+    if (j < blocks && ((j0 == b + 1 ? near : a.flags[j]) & kSpan) == 0u) atomicMin(&s_end, j);
     __syncthreads();
     const uint32_t end = s_end;
     __syncthreads();
     if (end < blocks) break;
   }
   const int heads = (int)(s_end - b);  // blocks b + 1 .. s_end
-  const int64_t per_block = (int64_t)a.groups * a.per_group;
-  const uint32_t key = a.keys[(b + 1) * per_block - 1];
   const int nv = (a.dim + 3) / 4, lanes = nv < kJoinThreads ? nv : kJoinThreads;
   int groups = kJoinThreads / lanes < kJoinGroups ? kJoinThreads / lanes : kJoinGroups;
   if (groups > (heads + kFlight - 1) / kFlight) groups = (heads + kFlight - 1) / kFlight;
@@ -784,26 +803,35 @@ bool sizes_ok(int64_t rows, int dim, int64_t n) {
   return rows >= 0 && rows <= 0x7FFFFFFE && dim >= 0 && dim <= kMaxDim && n >= 0 && n <= 0x7FFFFFFF;
 }
 
-template <typename T>
-int launch_rows(const void* table, int64_t rows, int dim, int64_t row_stride, const void* idx, int idx_bytes, int64_t n, float scale,
-                void* out, int64_t out_stride, hipStream_t stream) {
+template <typename T, typename I>
+int launch_rows(const void* table, int64_t rows, int dim, int64_t row_stride, const void* idx, int64_t n, float scale, void* out,
+                int64_t out_stride, hipStream_t stream) {
   constexpr int N = 16 / (int)sizeof(T);
   const uint32_t nv = (uint32_t)((dim + N - 1) / N);
   // l / nv = umulhi(l, magic) while l * nv < 2^32: l < nv + 1 024, nv <= 16 384
   const uint32_t magic = nv == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + nv - 1) / nv);
-  const dim3 grid((uint32_t)nr_cdiv(n * nv, kThreads * kRowUnroll));
-  if (idx_bytes == 8)
-    hipLaunchKernelGGL((rows_kernel<T, int64_t>), grid, dim3(kThreads), 0, stream, static_cast<const T*>(table), rows, dim, row_stride,
-                       static_cast<const int64_t*>(idx), n, scale, static_cast<T*>(out), out_stride, nv, magic);
-  else
-    hipLaunchKernelGGL((rows_kernel<T, int32_t>), grid, dim3(kThreads), 0, stream, static_cast<const T*>(table), rows, dim, row_stride,
-                       static_cast<const int32_t*>(idx), n, scale, static_cast<T*>(out), out_stride, nv, magic);
+  const bool past = n * dim * (int64_t)sizeof(T) > kStreamBytes;
+  auto kernel = past ? rows_kernel<T, I, true> : rows_kernel<T, I, false>;
+  hipLaunchKernelGGL(kernel, dim3((uint32_t)nr_cdiv(n * nv, kThreads * kRowUnroll)), dim3(kThreads), 0, stream, static_cast<const T*>(table),
+                     rows, dim, row_stride, static_cast<const I*>(idx), n, scale, static_cast<T*>(out), out_stride, nv, magic);
   NR_LAUNCH_CHECK();
   return 0;
 }
 
 template <typename I>
 int launch_sort(const Plan& p, SortPass s, const void* idx, uint32_t* const (&pairs)[4], hipStream_t stream) {
+  // zeros in equal shares, of whole vectors
+  uint16_t* zeros = s.zeros;
+  const int64_t halves = zeros != nullptr ? s.halves : 0, share = nr_cdiv(nr_cdiv(halves, 3 * p.passes), 8) * 8;
+  int64_t done = 0;
+  auto launch = [&](auto kernel, uint32_t blocks, auto... args) {
+    s.zeros = zeros + done;
+    s.halves = halves - done < share ? halves - done : share;
+    const int64_t want = nr_cdiv(s.halves, kThreads * 32);
+    s.zero_blocks = (uint32_t)(want < kZeroBlocks ? want : kZeroBlocks);
+    done += s.halves;
+    hipLaunchKernelGGL(kernel, dim3(blocks + s.zero_blocks), dim3(kThreads), 0, stream, s, args...);
+  };
   for (int pass = 0; pass < p.passes; ++pass) {
     s.shift = pass * p.digit_bits;
     s.bits = p.digit_bits;
@@ -811,9 +839,9 @@ int launch_sort(const Plan& p, SortPass s, const void* idx, uint32_t* const (&pa
     s.pos = pass == 0 ? nullptr : pairs[(pass - 1) % 2 * 2 + 1];
     s.keys_out = pairs[pass % 2 * 2];
     s.pos_out = pairs[pass % 2 * 2 + 1];
-    hipLaunchKernelGGL(sort_count_kernel<I>, dim3(p.sort_blocks), dim3(kThreads), 0, stream, s, static_cast<const I*>(idx));
-    hipLaunchKernelGGL(sort_scan_kernel, dim3((uint32_t)nr_cdiv(1 << s.bits, kScanDigits)), dim3(kThreads), 0, stream, s);
-    hipLaunchKernelGGL(sort_scatter_kernel<I>, dim3(p.sort_blocks), dim3(kThreads), 0, stream, s, static_cast<const I*>(idx));
+    launch(sort_count_kernel<I>, p.sort_blocks, static_cast<const I*>(idx));
+    launch(sort_scan_kernel, (uint32_t)nr_cdiv(1 << s.bits, kScanDigits));
+    launch(sort_scatter_kernel<I>, p.sort_blocks, static_cast<const I*>(idx));
     NR_LAUNCH_CHECK();
   }
   return 0;
@@ -831,7 +859,7 @@ int launch_sum(const Plan& p, const SumArgs& a, const void* grad, hipStream_t st
   return 0;
 }
 
-constexpr size_t own_lds(int vec, int rounds) { return (size_t)(2 * kOwnThreads * vec + rounds * kOwnThreads) * 4 + kOwnThreads; }
+constexpr size_t own_lds(int vec, int list_words) { return (size_t)(2 * kOwnThreads * vec + list_words) * 4 + kOwnThreads; }
 
 template <typename T, typename I>
 int launch_own(const OwnPlan& p, const OwnArgs& o, const void* grad, const void* idx, hipStream_t stream) {
@@ -839,8 +867,8 @@ int launch_own(const OwnPlan& p, const OwnArgs& o, const void* grad, const void*
   const dim3 grid((uint32_t)p.ranges, (uint32_t)p.col_tiles), block(kOwnThreads);
   const T* g = static_cast<const T*>(grad);
   const I* x = static_cast<const I*>(idx);
-  if (o.sum.n <= 2 * kOwnThreads) hipLaunchKernelGGL((own_kernel<T, I, 2>), grid, block, own_lds(N, 2), stream, o, g, x);
-  else hipLaunchKernelGGL((own_kernel<T, I, kOwnRounds>), grid, block, own_lds(N, kOwnRounds), stream, o, g, x);
+  if (o.sum.n <= 2 * kOwnThreads) hipLaunchKernelGGL((own_kernel<T, I, 2>), grid, block, own_lds(N, o.list_words), stream, o, g, x);
+  else hipLaunchKernelGGL((own_kernel<T, I, kOwnRounds>), grid, block, own_lds(N, o.list_words), stream, o, g, x);
   NR_LAUNCH_CHECK();
   return 0;
 }
@@ -848,10 +876,10 @@ int launch_own(const OwnPlan& p, const OwnArgs& o, const void* grad, const void*
 template <typename T>
 int init_own() {
   constexpr int N = 16 / (int)sizeof(T);
-  if (int rc = nr_raise_lds(own_kernel<T, int64_t, 2>, own_lds(N, 2))) return rc;
-  if (int rc = nr_raise_lds(own_kernel<T, int32_t, 2>, own_lds(N, 2))) return rc;
-  if (int rc = nr_raise_lds(own_kernel<T, int64_t, kOwnRounds>, own_lds(N, kOwnRounds))) return rc;
-  return nr_raise_lds(own_kernel<T, int32_t, kOwnRounds>, own_lds(N, kOwnRounds));
+  if (int rc = nr_raise_lds(own_kernel<T, int64_t, 2>, own_lds(N, 2 * kOwnThreads))) return rc;
+  if (int rc = nr_raise_lds(own_kernel<T, int32_t, 2>, own_lds(N, 2 * kOwnThreads))) return rc;
+  if (int rc = nr_raise_lds(own_kernel<T, int64_t, kOwnRounds>, own_lds(N, kOwnMax))) return rc;
+  return nr_raise_lds(own_kernel<T, int32_t, kOwnRounds>, own_lds(N, kOwnMax));
 }
 
 // Few indices go through the one-launch method; what it cannot hold in a list entry is sorted.
@@ -872,9 +900,11 @@ extern "C" int nr_embedding_fwd(const void* table, int dtype, int64_t rows, int 
   if (idx == nullptr || out == nullptr || (table == nullptr && rows > 0)) return NR_EINVAL;
   const int vec = 16 / dtype_size(dtype);
   if (nr_cdiv(n * ((dim + vec - 1) / vec), kThreads * kRowUnroll) > 0x7FFFFFFF) return NR_EINVAL;  // (blocks of one launch)
-  if (dtype == NR_DTYPE_F32) return launch_rows<float>(table, rows, dim, row_stride, idx, idx_bytes, n, scale, out, out_stride, nr_s(stream));
-  if (dtype == NR_DTYPE_BF16) return launch_rows<__bf16>(table, rows, dim, row_stride, idx, idx_bytes, n, scale, out, out_stride, nr_s(stream));
-  return launch_rows<_Float16>(table, rows, dim, row_stride, idx, idx_bytes, n, scale, out, out_stride, nr_s(stream));
+  const bool wide = idx_bytes == 8;
+  auto launch = dtype == NR_DTYPE_F32    ? (wide ? launch_rows<float, int64_t> : launch_rows<float, int32_t>)
+                : dtype == NR_DTYPE_BF16 ? (wide ? launch_rows<__bf16, int64_t> : launch_rows<__bf16, int32_t>)
+                                         : (wide ? launch_rows<_Float16, int64_t> : launch_rows<_Float16, int32_t>);
+  return launch(table, rows, dim, row_stride, idx, n, scale, out, out_stride, nr_s(stream));
 }
 
 extern "C" int64_t nr_embedding_bwd_workspace_bytes(int64_t rows, int dim, int64_t n, int grad_dtype) {
@@ -905,7 +935,7 @@ extern "C" int nr_embedding_bwd(const void* grad, int grad_dtype, int64_t grad_s
     const OwnPlan p = make_own_plan(rows, dim, dtype_size(grad_dtype));
     a.group = p.group;
     a.groups = p.groups;
-    const OwnArgs o = {a, padding, p.range, p.key_bits};
+    const OwnArgs o = {a, padding, p.range, p.key_bits, (int)((n + 63) / 64 * 64)};
     if (idx_bytes == 8)
       return grad_dtype == NR_DTYPE_F32 ? launch_own<float, int64_t>(p, o, grad, idx, st)
              : grad_dtype == NR_DTYPE_BF16 ? launch_own<__bf16, int64_t>(p, o, grad, idx, st) : launch_own<_Float16, int64_t>(p, o, grad, idx, st);
@@ -913,11 +943,10 @@ extern "C" int nr_embedding_bwd(const void* grad, int grad_dtype, int64_t grad_s
            : grad_dtype == NR_DTYPE_BF16 ? launch_own<__bf16, int32_t>(p, o, grad, idx, st) : launch_own<_Float16, int32_t>(p, o, grad, idx, st);
   }
   if (n > 0 && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0)) return NR_EINVAL;
-  if (!accumulate) {
-    // the whole table: rows that nothing looks up are zero
-    const int64_t halves = rows * dim * (dtype_size(table_dtype) / 2);
-    const int64_t blocks = nr_cdiv(halves, kThreads * 8);
-    hipLaunchKernelGGL(clear_kernel, dim3((uint32_t)(blocks < 4096 ? blocks : 4096)), dim3(kThreads), 0, st,
+  const int64_t halves = accumulate ? 0 : rows * dim * (dtype_size(table_dtype) / 2);  // zeros where nothing is looked up
+  if (n == 0 && halves > 0) {
+    const int64_t blocks = nr_cdiv(halves, kThreads * 32);
+    hipLaunchKernelGGL(clear_kernel, dim3((uint32_t)(blocks < kZeroBlocks ? blocks : kZeroBlocks)), dim3(kThreads), 0, st,
                        static_cast<uint16_t*>(grad_table), halves);
     NR_LAUNCH_CHECK();
   }
@@ -933,6 +962,8 @@ extern "C" int nr_embedding_bwd(const void* grad, int grad_dtype, int64_t grad_s
   s.rows = rows;
   s.padding = padding;
   s.blocks = p.sort_blocks;
+  s.zeros = static_cast<uint16_t*>(grad_table);
+  s.halves = halves;
   if (int rc = idx_bytes == 8 ? launch_sort<int64_t>(p, s, idx, pairs, st) : launch_sort<int32_t>(p, s, idx, pairs, st)) return rc;
   a.keys = pairs[(p.passes - 1) % 2 * 2];
   a.pos = pairs[(p.passes - 1) % 2 * 2 + 1];

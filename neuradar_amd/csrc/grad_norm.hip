@@ -147,7 +147,7 @@ norm_finish_kernel(const double* __restrict__ partial, int64_t count, double max
   }
 }
 
-template <typename T, typename O>
+template <typename T, typename O, bool STREAM>
 __device__ __forceinline__ void piece_scale(const T* __restrict__ x, O* __restrict__ y, int64_t lo, int64_t hi, float f) {
   constexpr int N = 16 / (int)sizeof(T), kStep = kThreads * N;
   int64_t i = lo + threadIdx.x * N;
@@ -159,7 +159,8 @@ __device__ __forceinline__ void piece_scale(const T* __restrict__ x, O* __restri
     for (int u = 0; u < kUnroll; ++u) {
 #pragma unroll
       for (int k = 0; k < N; ++k) v[u][k] *= f;
-      nr_store_pack<O, N>(y + i + u * kStep, v[u]);
+      if constexpr (STREAM) nr_store_pack_stream<O, N>(y + i + u * kStep, v[u]);
+      else nr_store_pack<O, N>(y + i + u * kStep, v[u]);
     }
   }
   for (; i < hi; i += kStep) {
@@ -171,13 +172,14 @@ __device__ __forceinline__ void piece_scale(const T* __restrict__ x, O* __restri
     nr_store_some<O, N>(y + i, m, v);
   }
 }
-template <typename T>
+template <typename T, bool STREAM>
 __device__ __forceinline__ void piece_scale_to(const T* x, void* y, int out_dtype, int64_t lo, int64_t hi, float f) {
-  if (out_dtype == NR_DTYPE_F32) piece_scale<T, float>(x, static_cast<float*>(y), lo, hi, f);
-  else if (out_dtype == NR_DTYPE_BF16) piece_scale<T, __bf16>(x, static_cast<__bf16*>(y), lo, hi, f);
-  else piece_scale<T, _Float16>(x, static_cast<_Float16*>(y), lo, hi, f);
+  if (out_dtype == NR_DTYPE_F32) piece_scale<T, float, STREAM>(x, static_cast<float*>(y), lo, hi, f);
+  else if (out_dtype == NR_DTYPE_BF16) piece_scale<T, __bf16, STREAM>(x, static_cast<__bf16*>(y), lo, hi, f);
+  else piece_scale<T, _Float16, STREAM>(x, static_cast<_Float16*>(y), lo, hi, f);
 }
 
+template <bool STREAM>
 __global__ void __launch_bounds__(kThreads)
 scale_kernel(List l, const float* __restrict__ result) {
   const float f = result[1];
@@ -187,9 +189,9 @@ scale_kernel(List l, const float* __restrict__ result) {
   if (f == 1.0f && l.in[t] == l.out[t]) return;  // in place and within the norm: nothing to do
   const int64_t lo = (int64_t)(block - l.first[t]) * l.piece;
   const int64_t hi = lo + l.piece < l.numel[t] ? lo + l.piece : l.numel[t];
-  if (l.in_dtype[t] == NR_DTYPE_F32) piece_scale_to(static_cast<const float*>(l.in[t]), l.out[t], l.out_dtype[t], lo, hi, f);
-  else if (l.in_dtype[t] == NR_DTYPE_BF16) piece_scale_to(static_cast<const __bf16*>(l.in[t]), l.out[t], l.out_dtype[t], lo, hi, f);
-  else piece_scale_to(static_cast<const _Float16*>(l.in[t]), l.out[t], l.out_dtype[t], lo, hi, f);
+  if (l.in_dtype[t] == NR_DTYPE_F32) piece_scale_to<float, STREAM>(static_cast<const float*>(l.in[t]), l.out[t], l.out_dtype[t], lo, hi, f);
+  else if (l.in_dtype[t] == NR_DTYPE_BF16) piece_scale_to<__bf16, STREAM>(static_cast<const __bf16*>(l.in[t]), l.out[t], l.out_dtype[t], lo, hi, f);
+  else piece_scale_to<_Float16, STREAM>(static_cast<const _Float16*>(l.in[t]), l.out[t], l.out_dtype[t], lo, hi, f);
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host
@@ -291,8 +293,12 @@ extern "C" int nr_grad_scale(const void* const* grads, void* const* outs, const 
   Cut c;
   if (!cut_list(numel, count, &c) || !list_ok(grads, numel, dtypes, count) || !list_ok(outs, numel, out_dtypes, count) || result == nullptr)
     return NR_EINVAL;
+  int64_t bytes = 0;
+  for (int t = 0; t < count; ++t) bytes += numel[t] * (out_dtypes[t] == NR_DTYPE_F32 ? 4 : 2);
+  const bool past = bytes > kStreamBytes;
   return for_each_run(grads, outs, numel, dtypes, out_dtypes, count, c, [&](const List& l, uint32_t blocks, int64_t) {
-    hipLaunchKernelGGL(scale_kernel, dim3(blocks), dim3(kThreads), 0, nr_s(stream), l, result);
+    if (past) hipLaunchKernelGGL(scale_kernel<true>, dim3(blocks), dim3(kThreads), 0, nr_s(stream), l, result);
+    else hipLaunchKernelGGL(scale_kernel<false>, dim3(blocks), dim3(kThreads), 0, nr_s(stream), l, result);
     NR_LAUNCH_CHECK();
     return 0;
   });
