@@ -1,4 +1,5 @@
-"""Drop-in `HashEncoding` / `SHEncoding` (reference: field_components/encodings.py:311-471,760-805).
+"""Drop-in `HashEncoding` / `SHEncoding` (reference: field_components/encodings.py:311-471,760-805) and `Embedding`
+(field_components/embedding.py).
 
 Same constructor arguments and attributes (`num_levels`, `features_per_level`, `scalings`,
 `hash_table` as an nn.Parameter in the torch layout [L*T, F]); `implementation="hip"` runs the
@@ -49,6 +50,28 @@ class HashEncoding(nn.Module):
         s = None if std is None else std.reshape(-1).contiguous()
         out = ops.hash_encode(x, self.hash_table, self.scalings, self.log2_hashmap_size, std=s)
         return out.view(*in_tensor.shape[:-1], self.get_out_dim())
+
+
+class Embedding(nn.Module):
+    """Rows by index (field_components/embedding.py: same arguments, `mean` and state-dict key): per-image or per-sensor codes,
+    classes, tokens.  Lookup and gradient run on ops.embedding: any table in fp32 / bf16 / fp16, a gradient without atomics.
+    scale multiplies every row; padding_idx: a row that gets no gradient (nn.Embedding's convention)."""
+
+    def __init__(self, in_dim: int, out_dim: int, scale: float = 1.0, padding_idx: Optional[int] = None) -> None:
+        super().__init__()
+        self.in_dim, self.out_dim = in_dim, out_dim
+        self.scale, self.padding_idx = scale, padding_idx
+        self.embedding = nn.Embedding(in_dim, out_dim, padding_idx=padding_idx)  # parameter container (name, init)
+
+    def get_out_dim(self) -> int:
+        return self.out_dim
+
+    def mean(self, dim: int = 0) -> Tensor:
+        return self.embedding.weight.mean(dim)
+
+    def forward(self, in_tensor: Tensor) -> Tensor:
+        """in_tensor: indices of any shape -> [*shape, out_dim]."""
+        return ops.embedding(self.embedding.weight, in_tensor, self.scale, self.padding_idx)
 
 
 class SHEncoding(nn.Module):

@@ -470,8 +470,17 @@ class FusedTrainStep:
         reducer (parallel.GradAllReducer, world > 1; needs `optimizers`): data-parallel step.  The main table's
         gradient is exchanged as (row, value) lists right after its scatter (reduce_sparse), the proposal table's
         dense SUM all-reduce is issued on its side stream when both proposal scatters are done and runs over
-        RCCL/xGMI beside the main chain, the small-parameter bucket last; Adam applies 1/world (DDP's mean)."""
+        RCCL/xGMI beside the main chain, the small-parameter bucket last; Adam applies 1/world (DDP's mean).
+
+        Optimizers with a max_norm clip a whole group's gradients: all of them then step behind the backward instead of
+        beside it (single GPU; with a reducer: reduce, then FlatAdam.step())."""
         lib, p, c, B = self.lib, ops._p, self.cfg, self.B
+        behind = None  # optimizers that step when every gradient is there
+        if optimizers is not None and any(getattr(o_, "max_norm", None) is not None for o_ in optimizers):
+            if reducer is not None:
+                raise NotImplementedError("an optimizer with max_norm cannot be fused with a reducer: call forward_backward without "
+                                          "optimizers, reducer.all_reduce() and the optimizers' step()")
+            behind, optimizers = optimizers, None
         st = ops._stream()
         assert self.C <= 32 and (target_features is None or target_features.shape[1] == self.C)
         if c.appearance_dim > 0 and self.dec is None and not any(
@@ -852,7 +861,8 @@ class FusedTrainStep:
                                        p(self.features), p(self.depth), st), "composite_fwd")
             if early == 5:
                 start_chains_before()
-            epoch = optimizers[0].step_t if optimizers is not None else None
+            stepping = optimizers if optimizers is not None else behind
+            epoch = stepping[0].step_t if stepping is not None else None
             g_f_extra, g_d_extra = self._timed("decoders", lambda: self.dec["head"].backward_into(
                 self.features, self.depth, times, self.dec["sensor_idx"], self.dec["batches"][slot], self.loss, seed_epoch=epoch))
             rgb_mult = depth_mult = 0.0
@@ -1042,6 +1052,14 @@ class FusedTrainStep:
         join_all()
         if optimizers is not None:
             small_and_other_steps()
+        if behind is not None:
+            for o_ in behind:
+                if o_ is not behind[0]:
+                    for i in range(len(o_.buffers)):
+                        o_.check_buffer(i)  # (the tables' gradients are flagged by the field backward)
+                o_.step()
+            if self.amp is not None:
+                self.amp.update()
         return self.loss
 
     def outputs(self) -> Dict[str, Tensor]:

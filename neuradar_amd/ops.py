@@ -1385,6 +1385,20 @@ def grad_norm(grads, norm_type: float = 2.0) -> Tensor:
     return _norm_and_factor(_GradList(grads, "gradients"), float("inf"), norm_type, device)[0]
 
 
+def clip_factor(grads, max_norm: float, norm_type: float = 2.0) -> Tuple[Tensor, Tensor]:
+    """(norm, min(1, max_norm / (norm + 1e-6))) as fp32 tensors of one element each, the gradients untouched: for an optimizer that
+    multiplies them itself (adam_step's `clip`), which saves the pass that clip_grads makes over them."""
+    grads = _as_list(grads)
+    if not grads:
+        raise RuntimeError("clip_factor: no gradients")
+    device = grads[0].device
+    if device.type == "cuda" and device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return clip_factor(grads, max_norm, norm_type)
+    result = _norm_and_factor(_GradList(grads, "gradients"), float(max_norm), norm_type, device)
+    return result[0:1], result[1:2]
+
+
 def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> Tensor:
     """Scale gradients by min(1, max_norm / (norm + 1e-6)), norm = grad_norm(grads, norm_type), which is returned.  In place, or
     into the tensors of `out` (as many elements each, any of the three types: places in a 16-bit bucket, say), one rounding.  Nothing is read on

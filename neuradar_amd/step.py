@@ -41,6 +41,9 @@ class HotPathConfig:
     single_jitter: bool = True
     static_scale: float = 100.0
     appearance_dim: int = 0  # 16 in the reference; the embedding lookup is a torch gather (neuradar.py:550-568)
+    # True: the modular model looks the appearance rows up with ops.embedding, whose gradient is summed by sorted indices (the
+    # same bits on every run); False: torch's gather and its backward
+    sorted_appearance_grad: bool = False
     duration: float = 20.0
     num_sensors: int = 1
     temporal_appearance_freq: float = 1.0
@@ -190,8 +193,11 @@ class NeuRadarHotPath(nn.Module):
         after = (before + 1).clamp(0, E - 1)
         ratio = time_idx - before
         before, after = before + sensor_idx * E, after + sensor_idx * E
-        e0 = self.appearance_embedding(before.squeeze(-1).long())
-        e1 = self.appearance_embedding(after.squeeze(-1).long())
+        look_up = self.appearance_embedding
+        if self.config.sorted_appearance_grad:
+            look_up = lambda idx: ops.embedding(self.appearance_embedding.weight, idx)  # noqa: E731
+        e0 = look_up(before.squeeze(-1).long())
+        e1 = look_up(after.squeeze(-1).long())
         return e0 * (1 - ratio) + e1 * ratio
 
     def get_nff_outputs(self, bundle: RayBundle, t_rand=None, jitters=(None, None), flips=(None, None, None)) -> Dict[str, Tensor]:
@@ -496,6 +502,11 @@ class FlatAdam:
     """Adam/AdamW with the fused HIP kernel.  Small parameters are re-homed into ONE flat buffer
     (views keep names/shapes), so a step is one launch for all of them plus one per hash table.
 
+    max_norm: clip the gradients of ALL this optimizer's parameters to a global norm before a step (the reference's
+    OptimizerConfig.max_norm: clip_grad_norm_ per parameter group, engine/optimizers.py).  The factor stays on the device and is
+    multiplied inside the Adam launches, so clipping costs one read of the gradients; `total_norm` holds the last step's norm.
+    The whole group has to be there first: `step()` only, not the buffers one by one (`step_buffer`), no sharded buffers.
+
     Hyper-parameters of configs/method_configs.py:384-409; the (lr, bias-correction) triple lives in a
     device tensor updated by a few scalar ops so that a captured graph can be replayed.  Parameters in
     `skip` never receive a gradient (proposal_fields[0], see NeuRadarHotPath) and are left untouched,
@@ -505,7 +516,11 @@ class FlatAdam:
 
     def __init__(self, params: List[nn.Parameter], lr: float, eps: float = 1e-15, weight_decay: float = 0.0,
                  adamw: bool = False, betas=(0.9, 0.999), lr_final: Optional[float] = None, max_steps: int = 20001,
-                 warmup_steps: int = 500, skip: Optional[List[nn.Parameter]] = None, flatten: bool = True) -> None:
+                 warmup_steps: int = 500, skip: Optional[List[nn.Parameter]] = None, flatten: bool = True,
+                 max_norm: Optional[float] = None) -> None:
+        if max_norm is not None and not max_norm >= 0.0:
+            raise ValueError(f"max_norm must not be negative or NaN: {max_norm}")
+        self.max_norm, self.total_norm = max_norm, None
         skip_ids = {id(p) for p in (skip or [])}
         self.params = [p for p in params if p.requires_grad and id(p) not in skip_ids]
         self.lr, self.eps, self.wd, self.adamw, self.betas = lr, eps, weight_decay, adamw, betas
@@ -584,6 +599,8 @@ class FlatAdam:
         gradient onto the owners and all-gathers the updated rows).  Moments and `seen` flags shrink to the shard (2 x 537 MB
         -> 2 x 67 MB per GPU for NeuRadar's main table on 8 GPUs).  Returns (lo, hi), or None when the buffer does not
         divide into world pieces of whole 16-byte groups (it then stays replicated)."""
+        if self.max_norm is not None:
+            raise RuntimeError("FlatAdam(max_norm=...): a sharded buffer's gradient is not on one rank, its norm would be a part")
         p, g = self.buffers[i]
         n = p.numel()
         if (world <= 1 and not force) or n % (world * 4) != 0:  # (force: a one-rank group that runs the collectives anyway -- tests)
@@ -626,12 +643,14 @@ class FlatAdam:
 
     @torch.no_grad()
     def step_buffer(self, i: int, grad_scale: float = 1.0, delta16: Optional[Tensor] = None, skip_extra: Optional[Tensor] = None,
-                    part: Optional[Tuple[int, int]] = None) -> None:
+                    part: Optional[Tuple[int, int]] = None, clip: Optional[Tensor] = None) -> None:
         """Adam on buffer i (after `advance()`), on the current stream.  grad_scale = 1/world turns the
         SUM all-reduce of the data-parallel ranks into DDP's mean without a separate pass.  delta16 (bf16, one per element of
         this rank's shard): the update also leaves as a rounded delta for the other replicas (GradAllReducer.shard_step).
         skip_extra: a second skip flag (device float; GradAllReducer.reduce_sparse's overflow flag, value 2 = skip and keep the
-        gradient): the loss scaler's found-inf flag, when one is attached and raised, takes precedence."""
+        gradient): the loss scaler's found-inf flag, when one is attached and raised, takes precedence.
+        clip: the group's clip factor (`step()` with max_norm)."""
+        self._needs_whole_group(clip)
         (p, g), (m, v) = self.buffers[i], self.state[i]
         lo_hi = getattr(self, "shards", {}).get(i)
         if lo_hi is not None:  # this rank's rows only (the rest of the gradient buffer is cleared by the exchange)
@@ -651,7 +670,11 @@ class FlatAdam:
             p, g, m, v = p.view(-1)[lo:hi], g.view(-1)[lo:hi], m.view(-1)[lo:hi], v.view(-1)[lo:hi]
             seen = None if seen is None else seen[lo // 4:hi // 4]
         ops.adam_step(p, g, m, v, self.lr, 1, self.betas, self.eps, self.wd, self.adamw, grad_scale=grad_scale,
-                      zero_grad=True, dev_hyper=self.hyper, seen_grad=seen, marked=marked, skip=skip, delta16=delta16)
+                      zero_grad=True, dev_hyper=self.hyper, seen_grad=seen, marked=marked, skip=skip, delta16=delta16, clip=clip)
+
+    def _needs_whole_group(self, clip: Optional[Tensor]) -> None:
+        if self.max_norm is not None and clip is None:
+            raise RuntimeError("FlatAdam(max_norm=...): the gradients of the whole group are clipped together, step a buffer through step()")
 
     @torch.no_grad()
     def step_buffer_split(self, i: int, phase: int, stamp: Tensor) -> None:
@@ -660,6 +683,7 @@ class FlatAdam:
         any time after `advance()`, e.g. beside the forward; phase 2 (the stamped groups) after the scatter.  No loss scaler, no
         shards, no weight decay: FusedTrainStep falls back to step_buffer otherwise."""
         (p, g), (m, v) = self.buffers[i], self.state[i]
+        self._needs_whole_group(None)
         assert self.amp is None and i not in getattr(self, "shards", {}) and self.seen[i] is not None and self.wd == 0.0
         ops.adam_step_split(p.view(-1), g.view(-1), m, v, self.betas, self.eps, 1.0, self.hyper, self.seen[i], stamp, self.step_t[1:], phase)
 
@@ -757,5 +781,8 @@ class FlatAdam:
         self.advance()
         if hasattr(self, "marked"):  # whoever calls step() wrote the gradients without marking `seen` (modular backward, a
             self.marked.clear()      # collective): only FusedTrainStep pairs its marking scatter with step_buffer()
+        clip = None
+        if self.max_norm is not None:
+            self.total_norm, clip = ops.clip_factor(self.grad_buffers(), self.max_norm)
         for i in range(len(self.buffers)):
-            self.step_buffer(i)
+            self.step_buffer(i, clip=clip)

@@ -75,3 +75,32 @@ def test_cpu_tensors_are_refused():
         ops.embedding_grad(torch.zeros(2, 2), idx, 4)
     with pytest.raises(RuntimeError, match="float32, bfloat16 or float16"):
         ops.grad_norm([table.double()])
+
+
+def test_clipping_needs_the_whole_group():
+    from neuradar_amd.step import FlatAdam
+
+    p = torch.nn.Parameter(torch.ones(8))
+    for bad in (-1.0, float("nan")):
+        with pytest.raises(ValueError, match="max_norm"):
+            FlatAdam([p], lr=1e-2, max_norm=bad)
+    opt = FlatAdam([p], lr=1e-2, max_norm=1.0)
+    with pytest.raises(RuntimeError, match="whole group"):
+        opt.step_buffer(0)
+    with pytest.raises(RuntimeError, match="whole group"):
+        opt.step_buffer_split(0, 1, None)
+    with pytest.raises(RuntimeError, match="shard"):
+        opt.shard_buffer(0, 0, 2)
+    with pytest.raises(RuntimeError, match="no gradients"):
+        ops.clip_factor([], 1.0)
+
+
+def test_embedding_module_mirrors_the_reference():
+    from neuradar_amd.encodings import Embedding
+
+    emb = Embedding(7, 3)
+    assert list(emb.state_dict()) == ["embedding.weight"] and emb.get_out_dim() == 3 and emb.in_dim == 7
+    assert torch.equal(emb.mean(dim=0), emb.embedding.weight.mean(0))
+    assert not bool(Embedding(7, 3, padding_idx=2).embedding.weight[2].any())
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        emb(torch.tensor([1, 2]))
