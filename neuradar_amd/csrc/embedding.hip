@@ -380,15 +380,15 @@ __device__ __forceinline__ int first_stop(const uint64_t* span, int g, int group
 
 // Head r <- head r + r + 1 + ... up to the first that does not hand its sum on: by doubling, every group at once, so that a row
 // whose tokens fill the block costs log2(groups) steps and not `groups` of them (256 groups of one lane: 54 -> 25 us).  All
-// threads call it, behind a barrier; `head`: this thread's columns of group 0.
+// threads call it, behind a barrier; `used`: groups with tokens; `head`: this thread's columns of group 0.
 template <int N>
-__device__ __forceinline__ void chain_heads(const uint64_t* span, int r, bool work, int groups, float* head, int step) {
+__device__ __forceinline__ void chain_heads(const uint64_t* span, int r, bool work, int groups, int used, float* head, int step) {
   uint64_t any = 0ull;
   for (int w = 0; w * NR_WAVE < groups; ++w) any |= span[w];
   if (any == 0ull) return;
   const int run = work ? first_stop(span, r, groups) - r : 0;  // groups from r on that hand on
   float* own = head + r * step;
-  for (int d = 1; d < groups; d *= 2) {
+  for (int d = 1; d < used; d *= 2) {
     const bool add = work && run >= d && r + d < groups;
     float x[N];
     if (add)
@@ -449,7 +449,7 @@ sum_kernel(SumArgs a, const T* __restrict__ grad) {
   __syncthreads();
   mark_spans(s_flag, a.groups, s_span);
   __syncthreads();
-  chain_heads<N>(s_span, r, work, a.groups, s_head + lane * N, step);
+  chain_heads<N>(s_span, r, work, a.groups, (count + a.per_group - 1) / a.per_group, s_head + lane * N, step);
   // sums that cross stretches: their first group adds the parts behind it.  Group 0 also takes a sum that came in from the
   // block before.
   if (work) {
@@ -484,19 +484,27 @@ sum_kernel(SumArgs a, const T* __restrict__ grad) {
   }
 }
 
-// -------------------------------------------------------------------------------------------------- few indices: one launch
-// Up to kOwnMax indices: no sort of the whole, no workspace.  A block OWNS a range of rows (and of columns): it reads all
-// indices, keeps those of its range in ascending position (one ballot per 64), orders that short list by row, and sums it as
-// above; the rows of its range that nothing looks up it clears itself.  The indices are read by every block (128 KB from L2 at
-// 16 384 of 8 bytes), which is what limits the method to few of them.  A list is as long as the range's share of the tokens:
-// 64 on average, all of them at worst -- then one block per column range does the work, which is why columns are split
-// down to 64 bytes where there are fewer rows than blocks to fill the chip with.
+// ------------------------------------------------------------------------------------------- few indices, or a small table
+// No sort of the whole.  A block OWNS a range of rows (and of columns): it reads the indices, keeps those of its range in
+// ascending position (one ballot per 64), orders that short list by row, and sums it as above; the rows of its range that
+// nothing looks up it clears itself.  The indices are read by every block (128 KB from L2 at 16 384 of 8 bytes), and its list has
+// to fit into LDS, which limits the method to kOwnMax of them: one launch, no workspace.  More indices are taken in chunks, each
+// into a table of its own, in fp32; a second launch adds those in order -- where they are small (kOwnTables): two launches
+// instead of five or eight.
+// A list is as long as the range's share of the tokens: 64 on average, all of them at worst, and then a block per column range
+// does a chunk's work.  So columns are split down to 64 bytes, and the chunks down to 2 048, where there are fewer rows than
+// blocks to fill the chip with.
 constexpr int kOwnThreads = 1024;
 constexpr int kOwnRounds = 16;
 constexpr int kOwnMax = kOwnThreads * kOwnRounds;  // 14 bits of position, 18 of row in a list entry
 constexpr int kOwnPosBits = 14;
 constexpr int kOwnRangeMax = 1 << (32 - kOwnPosBits - 1);
 constexpr int kOwnBlocks = 256;
+constexpr int kOwnLanes = 32;    // half a kilobyte of a row per block at most (a kilobyte: 40 % slower where one row has a fifth of
+                                 // the tokens, 64 bytes: 30 % slower where all have the same share; 4 096 rows of 1 024 in bf16)
+constexpr int kOwnSplit = 65536; // bytes of gradient that a block sums at most, on average, before a chunk is cut
+constexpr int64_t kOwnTables = (int64_t)64 << 20;  // bytes of the chunks' tables: at 78 MB as fast as the sort (260 000 tokens on
+                                                   // 20 000 rows of 64 in fp32: 64 us against 74), far below it two or three times as fast
 constexpr int kCountSort = 256;  // lists up to this length: every entry counts the smaller ones
 constexpr int kOwnDigitBits = 8;
 
@@ -504,21 +512,26 @@ struct OwnArgs {
   SumArgs sum;
   int64_t padding;
   int range, key_bits;  // rows per block; bits of a row inside its range
-  int list_words;       // n, rounded up
+  int chunk, rounds;    // tokens per blockIdx.z, a multiple of 64; rounds of kOwnThreads that they take
 };
 
-template <typename T, typename I, int ROUNDS>
+template <typename T, typename I>
 __global__ void __launch_bounds__(kOwnThreads)
 own_kernel(OwnArgs o, const T* __restrict__ grad, const I* __restrict__ idx) {
   constexpr int N = 16 / (int)sizeof(T), kWaves = kOwnThreads / NR_WAVE;
-  const SumArgs& a = o.sum;
+  SumArgs a = o.sum;
+  const int64_t base = (int64_t)blockIdx.z * o.chunk;
+  const int n = a.n - base < o.chunk ? (int)(a.n - base) : o.chunk;
+  grad += base * a.grad_stride;
+  idx += base;
+  if (gridDim.z > 1) a.out = static_cast<float*>(a.out) + (int64_t)blockIdx.z * a.rows * a.dim;  // (partial tables, in fp32)
   extern __shared__ uint32_t lds[];
   const int step = a.group * N, lane = nr_lane(), wave = threadIdx.x / NR_WAVE;
   float* s_head = reinterpret_cast<float*>(lds);             // [groups][group * N]
   float* s_tail = s_head + a.groups * step;
   uint32_t* s_digit = lds;                                   // [waves][256]: before the sums
-  uint32_t* s_list = lds + 2 * kOwnThreads * N;              // [list_words]
-  unsigned char* s_flag = reinterpret_cast<unsigned char*>(s_list + o.list_words);  // [groups]
+  uint32_t* s_list = lds + 2 * kOwnThreads * N;              // [chunk]
+  unsigned char* s_flag = reinterpret_cast<unsigned char*>(s_list + o.chunk);  // [groups]
   __shared__ uint32_t s_count[kWaves];
   __shared__ uint64_t s_span[kWaves];
   const int64_t row0 = (int64_t)blockIdx.x * o.range;
@@ -527,13 +540,13 @@ own_kernel(OwnArgs o, const T* __restrict__ grad, const I* __restrict__ idx) {
   const int col = (blockIdx.y * a.group + glane) * N;
   const bool work = r < a.groups && col < a.dim;
 
-  uint32_t item[ROUNDS];
+  uint32_t item[kOwnRounds];
   constexpr uint32_t kNone = 0xFFFFFFFFu;
 #pragma unroll
-  for (int u = 0; u < ROUNDS; ++u) {
-    const int i = wave * (NR_WAVE * ROUNDS) + u * NR_WAVE + lane;
+  for (int u = 0; u < kOwnRounds; ++u) {
     item[u] = kNone;
-    if (i < a.n) {
+    const int i = wave * (NR_WAVE * o.rounds) + u * NR_WAVE + lane;
+    if (u < o.rounds && i < n) {
       const int64_t v = (int64_t)idx[i];
       if (v >= row0 && v < row0 + range && v != o.padding) item[u] = ((uint32_t)(v - row0) << kOwnPosBits) | (uint32_t)i;
     }
@@ -553,7 +566,7 @@ own_kernel(OwnArgs o, const T* __restrict__ grad, const I* __restrict__ idx) {
   }
   uint32_t mine = 0u;
 #pragma unroll
-  for (int u = 0; u < ROUNDS; ++u) mine += (uint32_t)__popcll(__ballot(item[u] != kNone));
+  for (int u = 0; u < kOwnRounds; ++u) mine += (uint32_t)__popcll(__ballot(item[u] != kNone));
   if (lane == 0) s_count[wave] = mine;
   __syncthreads();
   uint32_t at = 0u, total = 0u;
@@ -565,7 +578,8 @@ own_kernel(OwnArgs o, const T* __restrict__ grad, const I* __restrict__ idx) {
   const int m = (int)total;
   if (m == 0) return;
 #pragma unroll
-  for (int u = 0; u < ROUNDS; ++u) {
+  for (int u = 0; u < kOwnRounds; ++u) {
+    if (u >= o.rounds) break;
     const uint64_t hit = __ballot(item[u] != kNone);
     if (item[u] != kNone) s_list[at + (uint32_t)__popcll(hit & ((1ull << lane) - 1ull))] = item[u];
     at += (uint32_t)__popcll(hit);
@@ -587,15 +601,15 @@ own_kernel(OwnArgs o, const T* __restrict__ grad, const I* __restrict__ idx) {
     for (int shift = 0; shift < o.key_bits; shift += kOwnDigitBits) {
       constexpr int kDigits = 1 << kOwnDigitBits;
       for (int d = threadIdx.x; d < kWaves * kDigits; d += kOwnThreads) s_digit[d] = 0u;
-      uint32_t rank[ROUNDS];
+      uint32_t rank[kOwnRounds];
 #pragma unroll
-      for (int u = 0; u < ROUNDS; ++u) {
-        const int i = wave * (NR_WAVE * ROUNDS) + u * NR_WAVE + lane;
-        item[u] = i < m ? s_list[i] : kNone;
+      for (int u = 0; u < kOwnRounds; ++u) {
+        const int i = wave * (NR_WAVE * o.rounds) + u * NR_WAVE + lane;
+        item[u] = u < o.rounds && i < m ? s_list[i] : kNone;
       }
       __syncthreads();
 #pragma unroll
-      for (int u = 0; u < ROUNDS; ++u) {
+      for (int u = 0; u < kOwnRounds; ++u) {
         const bool in = item[u] != kNone;
         const uint32_t d = (item[u] >> (kOwnPosBits + shift)) & (kDigits - 1);
         uint64_t peers = __ballot(in);
@@ -648,7 +662,7 @@ own_kernel(OwnArgs o, const T* __restrict__ grad, const I* __restrict__ idx) {
       }
       __syncthreads();
 #pragma unroll
-      for (int u = 0; u < ROUNDS; ++u) {
+      for (int u = 0; u < kOwnRounds; ++u) {
         if (item[u] == kNone) continue;
         const uint32_t d = (item[u] >> (kOwnPosBits + shift)) & (kDigits - 1);
         s_list[s_first[d] + s_digit[wave * kDigits + d] + rank[u]] = item[u];
@@ -672,13 +686,43 @@ own_kernel(OwnArgs o, const T* __restrict__ grad, const I* __restrict__ idx) {
   __syncthreads();
   mark_spans(s_flag, a.groups, s_span);
   __syncthreads();
-  chain_heads<N>(s_span, r, work, a.groups, s_head + glane * N, step);
+  chain_heads<N>(s_span, r, work, a.groups, (m + per - 1) / per, s_head + glane * N, step);
   if (work && (s_flag[r] & kTail)) {  // (the last token's sum ends with the list: a group follows)
     float acc[N];
 #pragma unroll
     for (int k = 0; k < N; ++k) acc[k] = tail[k] + head[step + k];
     write_row<N>(a, (uint32_t)row0 + key_at(q1 - 1), col, acc);
   }
+}
+
+// out (+)= round(scale * (tables[0] + tables[1] + ...)), 4 elements per thread
+template <typename O>
+__global__ void __launch_bounds__(kThreads)
+merge_kernel(const float* __restrict__ tables, int chunks, int64_t elements, float scale, int accumulate, O* __restrict__ out) {
+  const int64_t i = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * 4;
+  if (i >= elements) return;
+  const int m = elements - i < 4 ? (int)(elements - i) : 4;
+  float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int c = 0; c < chunks; c += kFlight) {
+    float x[kFlight][4];
+#pragma unroll
+    for (int u = 0; u < kFlight; ++u)
+      if (c + u < chunks) nr_load_some<float, 4>(tables + (c + u) * elements + i, m, x[u]);
+#pragma unroll
+    for (int u = 0; u < kFlight; ++u)
+      if (c + u < chunks)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[k] += x[u][k];
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) acc[k] *= scale;
+  if (accumulate) {
+    float was[4];
+    nr_load_some<O, 4>(out + i, m, was);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) acc[k] += was[k];
+  }
+  nr_store_some<O, 4>(out + i, m, acc);
 }
 
 // A sum that starts in block b and leaves it: tail[b] + head[b + 1] + ... + the head that ends it.  A row that thousands of
@@ -787,24 +831,41 @@ Plan make_plan(int64_t rows, int dim, int64_t n, int elem_size) {
   return p;
 }
 
-// The one-launch method: how many columns and rows a block owns.
+// Owners: how many columns, rows and tokens a block takes.  chunks == 0: the tokens are sorted instead.
 struct OwnPlan {
-  int group, groups, col_tiles, range, ranges, key_bits;
+  int group, groups, col_tiles, range, ranges, key_bits, chunk, chunks;
 };
-OwnPlan make_own_plan(int64_t rows, int dim, int elem_size) {
+OwnPlan make_own_plan(int64_t rows, int dim, int64_t n, int elem_size) {
   OwnPlan p = {};
+  if (rows > (int64_t)kOwnRangeMax * kOwnBlocks) return p;  // (18 bits of a list entry for the row)
   const int vec = 16 / elem_size, nv = (dim + vec - 1) / vec;
-  int lanes = nv < NR_WAVE ? nv : NR_WAVE;  // a kilobyte of a row, then down to 64 bytes while there are CUs without a block
-  while (lanes > 4 && rows * ((nv + lanes - 1) / lanes) < kOwnBlocks) lanes = (lanes + 1) / 2;
-  p.col_tiles = (nv + lanes - 1) / lanes;
+  auto cut = [&](int chunk) {
+    p.chunk = chunk;
+    p.chunks = (int)nr_cdiv(n, chunk);
+    const int blocks = p.chunks < kOwnBlocks ? (kOwnBlocks + p.chunks - 1) / p.chunks : 1;
+    int lanes = nv < kOwnLanes ? nv : kOwnLanes;  // half a kilobyte of a row, then down to 64 bytes while there are CUs without a block
+    while (lanes > 4 && rows * ((nv + lanes - 1) / lanes) < blocks) lanes = (lanes + 1) / 2;
+    p.col_tiles = (nv + lanes - 1) / lanes;
+    const int64_t want = p.col_tiles < blocks ? (blocks + p.col_tiles - 1) / p.col_tiles : 1;
+    int64_t range = nr_cdiv(rows, want);
+    if (range > kOwnRangeMax) range = kOwnRangeMax;
+    p.range = (int)range;
+    p.ranges = (int)nr_cdiv(rows, range);
+  };
+  cut(n < kOwnMax ? (int)(nr_cdiv(n, NR_WAVE) * NR_WAVE) : kOwnMax);
+  // few rows, or wide ones: their tokens on more blocks.  (In one chunk only where a block has much to read: a second launch
+  // costs 3 us.  16 384 tokens on one row of 1 024: 56 -> 34 us)
+  auto per_block = [&] { return nr_cdiv(p.chunk, p.ranges) * nr_cdiv(nv, p.col_tiles) * 16; };
+  if (p.chunks > 1 || per_block() > kOwnSplit)
+    while (p.chunk > 2048 && p.ranges * p.col_tiles * p.chunks < kOwnBlocks) cut(p.chunk > 4096 ? p.chunk / 128 * 64 : 2048);
+  if (p.chunks > 1 && p.chunks * rows * dim * (int64_t)sizeof(float) > kOwnTables) {
+    if (n <= kOwnMax) cut((int)(nr_cdiv(n, NR_WAVE) * NR_WAVE));  // (one chunk needs no tables)
+    else p.chunks = 0;
+  }
+  if (p.chunks > 65535) p.chunks = 0;
   p.group = (nv + p.col_tiles - 1) / p.col_tiles;
   p.groups = kOwnThreads / p.group;
-  const int64_t want = p.col_tiles < kOwnBlocks ? (kOwnBlocks + p.col_tiles - 1) / p.col_tiles : 1;
-  int64_t range = (rows + want - 1) / want;
-  if (range > kOwnRangeMax) range = kOwnRangeMax;
-  p.range = (int)range;
-  p.ranges = (int)((rows + range - 1) / range);
-  while (((range - 1) >> p.key_bits) != 0) ++p.key_bits;
+  while (((p.range - 1) >> p.key_bits) != 0) ++p.key_bits;
   return p;
 }
 
@@ -873,11 +934,8 @@ constexpr size_t own_lds(int vec, int list_words) { return (size_t)(2 * kOwnThre
 template <typename T, typename I>
 int launch_own(const OwnPlan& p, const OwnArgs& o, const void* grad, const void* idx, hipStream_t stream) {
   constexpr int N = 16 / (int)sizeof(T);
-  const dim3 grid((uint32_t)p.ranges, (uint32_t)p.col_tiles), block(kOwnThreads);
-  const T* g = static_cast<const T*>(grad);
-  const I* x = static_cast<const I*>(idx);
-  if (o.sum.n <= 2 * kOwnThreads) hipLaunchKernelGGL((own_kernel<T, I, 2>), grid, block, own_lds(N, o.list_words), stream, o, g, x);
-  else hipLaunchKernelGGL((own_kernel<T, I, kOwnRounds>), grid, block, own_lds(N, o.list_words), stream, o, g, x);
+  hipLaunchKernelGGL((own_kernel<T, I>), dim3((uint32_t)p.ranges, (uint32_t)p.col_tiles, (uint32_t)p.chunks), dim3(kOwnThreads),
+                     own_lds(N, o.chunk), stream, o, static_cast<const T*>(grad), static_cast<const I*>(idx));
   NR_LAUNCH_CHECK();
   return 0;
 }
@@ -885,14 +943,17 @@ int launch_own(const OwnPlan& p, const OwnArgs& o, const void* grad, const void*
 template <typename T>
 int init_own() {
   constexpr int N = 16 / (int)sizeof(T);
-  if (int rc = nr_raise_lds(own_kernel<T, int64_t, 2>, own_lds(N, 2 * kOwnThreads))) return rc;
-  if (int rc = nr_raise_lds(own_kernel<T, int32_t, 2>, own_lds(N, 2 * kOwnThreads))) return rc;
-  if (int rc = nr_raise_lds(own_kernel<T, int64_t, kOwnRounds>, own_lds(N, kOwnMax))) return rc;
-  return nr_raise_lds(own_kernel<T, int32_t, kOwnRounds>, own_lds(N, kOwnMax));
+  if (int rc = nr_raise_lds(own_kernel<T, int64_t>, own_lds(N, kOwnMax))) return rc;
+  return nr_raise_lds(own_kernel<T, int32_t>, own_lds(N, kOwnMax));
 }
 
-// Few indices go through the one-launch method; what it cannot hold in a list entry is sorted.
-bool owns(int64_t rows, int64_t n) { return n <= kOwnMax && rows <= (int64_t)kOwnRangeMax * kOwnBlocks; }
+template <typename O>
+int launch_merge(const OwnPlan& p, const float* tables, int64_t elements, float scale, int accumulate, void* out, hipStream_t stream) {
+  hipLaunchKernelGGL(merge_kernel<O>, dim3((uint32_t)nr_cdiv(elements, kThreads * 4)), dim3(kThreads), 0, stream, tables, p.chunks, elements,
+                     scale, accumulate, static_cast<O*>(out));
+  NR_LAUNCH_CHECK();
+  return 0;
+}
 
 }  // namespace
 
@@ -918,7 +979,10 @@ extern "C" int nr_embedding_fwd(const void* table, int dtype, int64_t rows, int 
 
 extern "C" int64_t nr_embedding_bwd_workspace_bytes(int64_t rows, int dim, int64_t n, int grad_dtype) {
   if (!dtype_ok(grad_dtype) || !sizes_ok(rows, dim, n)) return NR_EINVAL;
-  if (n == 0 || dim == 0 || rows == 0 || owns(rows, n)) return 0;
+  if (n == 0 || dim == 0 || rows == 0) return 0;
+  const OwnPlan own = make_own_plan(rows, dim, n, dtype_size(grad_dtype));
+  if (own.chunks == 1) return 0;
+  if (own.chunks > 1) return own.chunks * rows * dim * (int64_t)sizeof(float);
   return make_plan(rows, dim, n, dtype_size(grad_dtype)).bytes;
 }
 
@@ -940,18 +1004,27 @@ extern "C" int nr_embedding_bwd(const void* grad, int grad_dtype, int64_t grad_s
   a.out = grad_table;
   a.out_dtype = table_dtype;
   a.accumulate = accumulate;
-  if (n > 0 && owns(rows, n)) {
-    const OwnPlan p = make_own_plan(rows, dim, dtype_size(grad_dtype));
-    a.group = p.group;
-    a.groups = p.groups;
-    const OwnArgs o = {a, padding, p.range, p.key_bits, (int)((n + 63) / 64 * 64)};
-    if (idx_bytes == 8)
-      return grad_dtype == NR_DTYPE_F32 ? launch_own<float, int64_t>(p, o, grad, idx, st)
-             : grad_dtype == NR_DTYPE_BF16 ? launch_own<__bf16, int64_t>(p, o, grad, idx, st) : launch_own<_Float16, int64_t>(p, o, grad, idx, st);
-    return grad_dtype == NR_DTYPE_F32 ? launch_own<float, int32_t>(p, o, grad, idx, st)
-           : grad_dtype == NR_DTYPE_BF16 ? launch_own<__bf16, int32_t>(p, o, grad, idx, st) : launch_own<_Float16, int32_t>(p, o, grad, idx, st);
+  const OwnPlan own = n > 0 ? make_own_plan(rows, dim, n, dtype_size(grad_dtype)) : OwnPlan{};
+  if (n > 0 && own.chunks != 1 && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0)) return NR_EINVAL;
+  if (own.chunks > 0) {
+    a.group = own.group;
+    a.groups = own.groups;
+    if (own.chunks > 1) {
+      a.out = workspace;
+      a.out_dtype = NR_DTYPE_F32;
+      a.accumulate = 0;
+      a.scale = 1.0f;
+    }
+    const OwnArgs o = {a, padding, own.range, own.key_bits, own.chunk, (own.chunk + kOwnThreads - 1) / kOwnThreads};
+    const bool wide = idx_bytes == 8;
+    auto launch = grad_dtype == NR_DTYPE_F32    ? (wide ? launch_own<float, int64_t> : launch_own<float, int32_t>)
+                  : grad_dtype == NR_DTYPE_BF16 ? (wide ? launch_own<__bf16, int64_t> : launch_own<__bf16, int32_t>)
+                                                : (wide ? launch_own<_Float16, int64_t> : launch_own<_Float16, int32_t>);
+    if (int rc = launch(own, o, grad, idx, st)) return rc;
+    if (own.chunks == 1) return 0;
+    auto merge = table_dtype == NR_DTYPE_F32 ? launch_merge<float> : table_dtype == NR_DTYPE_BF16 ? launch_merge<__bf16> : launch_merge<_Float16>;
+    return merge(own, static_cast<const float*>(workspace), rows * dim, scale, accumulate, grad_table, st);
   }
-  if (n > 0 && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0)) return NR_EINVAL;
   const int64_t halves = accumulate ? 0 : rows * dim * (dtype_size(table_dtype) / 2);  // zeros where nothing is looked up
   if (n == 0 && halves > 0) {
     const int64_t blocks = nr_cdiv(halves, kThreads * 32);
