@@ -542,13 +542,14 @@ own_kernel(OwnArgs o, const T* __restrict__ grad, const I* __restrict__ idx) {
 
   uint32_t item[kOwnRounds];
   constexpr uint32_t kNone = 0xFFFFFFFFu;
+  const uint32_t padding = o.padding >= row0 && o.padding < row0 + range ? (uint32_t)(o.padding - row0) : kNone;
 #pragma unroll
   for (int u = 0; u < kOwnRounds; ++u) {
     item[u] = kNone;
     const int i = wave * (NR_WAVE * o.rounds) + u * NR_WAVE + lane;
     if (u < o.rounds && i < n) {
-      const int64_t v = (int64_t)idx[i];
-      if (v >= row0 && v < row0 + range && v != o.padding) item[u] = ((uint32_t)(v - row0) << kOwnPosBits) | (uint32_t)i;
+      const uint64_t d = (uint64_t)((int64_t)idx[i] - row0);  // (below the range: far above it)
+      if (d < (uint64_t)range && (uint32_t)d != padding) item[u] = ((uint32_t)d << kOwnPosBits) | (uint32_t)i;
     }
   }
   if (!a.accumulate) {  // all rows of the range; those that are looked up are written again below, behind the barriers
@@ -598,14 +599,15 @@ own_kernel(OwnArgs o, const T* __restrict__ grad, const I* __restrict__ idx) {
     __syncthreads();
   } else if (range > 1) {
     // by 8 bits of the row at a time, as in sort_scatter_kernel: the list through registers and back
+    const int rounds = (m + kOwnThreads - 1) / kOwnThreads;
     for (int shift = 0; shift < o.key_bits; shift += kOwnDigitBits) {
       constexpr int kDigits = 1 << kOwnDigitBits;
       for (int d = threadIdx.x; d < kWaves * kDigits; d += kOwnThreads) s_digit[d] = 0u;
       uint32_t rank[kOwnRounds];
 #pragma unroll
       for (int u = 0; u < kOwnRounds; ++u) {
-        const int i = wave * (NR_WAVE * o.rounds) + u * NR_WAVE + lane;
-        item[u] = u < o.rounds && i < m ? s_list[i] : kNone;
+        const int i = wave * (NR_WAVE * rounds) + u * NR_WAVE + lane;
+        item[u] = u < rounds && i < m ? s_list[i] : kNone;
       }
       __syncthreads();
 #pragma unroll
