@@ -11,6 +11,7 @@ from ctypes import POINTER, Structure, c_char_p, c_double, c_float, c_int, c_int
 
 CSRC = os.path.join(os.path.dirname(os.path.abspath(__file__)), "csrc")
 LIB_PATH = os.environ.get("NR_LIB_PATH") or os.path.join(CSRC, "libneuradar_hip.so")  # (NR_LIB_PATH: A/B runs of two builds)
+TENSORS_PATH = os.path.join(CSRC, "libneuradar_tensors.so")  # (host code against the installed torch: csrc/tensor_list.cpp)
 NR_MAX_LAYERS = 8
 NR_EINVAL = -1
 NR_LOSS_SLOTS = 1024
@@ -222,15 +223,15 @@ _lib = None
 
 def build(force: bool = False) -> str:
     """Compile the HIP library for gfx950 in-tree (hipcc cross-compiles without a GPU).  force: every file, whatever is built."""
-    if force or not os.path.exists(LIB_PATH) or _stale():
+    if force or not os.path.exists(LIB_PATH) or not os.path.exists(TENSORS_PATH) or _stale():
         subprocess.check_call(["make", "-C", CSRC, "-j8"] + (["-B"] if force else []), stdout=subprocess.DEVNULL)
     return LIB_PATH
 
 
 def _stale() -> bool:
-    so = os.path.getmtime(LIB_PATH)
+    so = min(os.path.getmtime(LIB_PATH), os.path.getmtime(TENSORS_PATH))
     inc = os.path.join(os.path.dirname(CSRC), "..", "include", "neuradar_hip.h")
-    srcs = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".hip", ".h"))] + [inc]
+    srcs = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".hip", ".h", ".cpp"))] + [inc]
     return any(os.path.getmtime(s) > so for s in srcs if os.path.exists(s))
 
 
@@ -258,6 +259,22 @@ def lib() -> ctypes.CDLL:
                     raise RuntimeError(f"{env}={value}: nr_set_tuning refused it")
         _lib = handle
     return _lib
+
+
+_tensors = None
+
+
+def tensors() -> ctypes.PyDLL:
+    """libneuradar_tensors.so: nr_tensor_list and nr_same_address (csrc/tensor_list.cpp), called with the interpreter lock held."""
+    global _tensors
+    if _tensors is None:
+        if not os.path.exists(TENSORS_PATH):
+            raise RuntimeError(f"{TENSORS_PATH} is missing. Build it with `make -C neuradar_amd/csrc`.")
+        handle = ctypes.PyDLL(TENSORS_PATH)
+        handle.nr_tensor_list.argtypes = [ctypes.py_object, P, P, P]
+        handle.nr_same_address.argtypes = [P, L]
+        _tensors = handle
+    return _tensors
 
 
 # nr_set_tuning knobs (include/neuradar_hip.h, NR_TUNE_*), in enum order: (environment variable forwarded at load, meaning)

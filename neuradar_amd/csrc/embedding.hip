@@ -750,7 +750,7 @@ join_kernel(SumArgs a, uint32_t blocks) {
     __syncthreads();
     if (end < blocks) break;
   }
-  const int heads = (int)(s_end - b);  // blocks b + 1 .. s_end
+  const int heads = (int)((s_end < blocks ? s_end : blocks - 1) - b);  // blocks b + 1 .. s_end (every sum ends: the last token's with it)
   const int nv = (a.dim + 3) / 4, lanes = nv < kJoinThreads ? nv : kJoinThreads;
   int groups = kJoinThreads / lanes < kJoinGroups ? kJoinThreads / lanes : kJoinGroups;
   if (groups > (heads + kFlight - 1) / kFlight) groups = (heads + kFlight - 1) / kFlight;
@@ -796,6 +796,7 @@ clear_kernel(uint16_t* __restrict__ p, int64_t halves) {
 // ---------------------------------------------------------------------------------------------------------------- host
 int dtype_size(int dtype) { return dtype == NR_DTYPE_F32 ? 4 : 2; }
 bool dtype_ok(int dtype) { return dtype == NR_DTYPE_F32 || dtype == NR_DTYPE_BF16 || dtype == NR_DTYPE_F16; }
+bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(bytes - 1)) == 0; }
 
 struct Plan {
   int bits, passes, digit_bits;
@@ -860,7 +861,7 @@ OwnPlan make_own_plan(int64_t rows, int dim, int64_t n, int elem_size) {
   auto per_block = [&] { return nr_cdiv(p.chunk, p.ranges) * nr_cdiv(nv, p.col_tiles) * 16; };
   if (p.chunks > 1 || per_block() > kOwnSplit)
     while (p.chunk > 2048 && p.ranges * p.col_tiles * p.chunks < kOwnBlocks) cut(p.chunk > 4096 ? p.chunk / 128 * 64 : 2048);
-  if (p.chunks > 1 && p.chunks * rows * dim * (int64_t)sizeof(float) > kOwnTables) {
+  if (p.chunks > 1 && (double)p.chunks * (double)rows * dim * sizeof(float) > (double)kOwnTables) {
     if (n <= kOwnMax) cut((int)(nr_cdiv(n, NR_WAVE) * NR_WAVE));  // (one chunk needs no tables)
     else p.chunks = 0;
   }
@@ -970,6 +971,7 @@ extern "C" int nr_embedding_fwd(const void* table, int dtype, int64_t rows, int 
   if (!dtype_ok(dtype) || !sizes_ok(rows, dim, n) || (idx_bytes != 4 && idx_bytes != 8) || row_stride < 0 || out_stride < dim) return NR_EINVAL;
   if (n == 0 || dim == 0) return 0;
   if (idx == nullptr || out == nullptr || (table == nullptr && rows > 0)) return NR_EINVAL;
+  if (!aligned(idx, idx_bytes) || !aligned(table, dtype_size(dtype)) || !aligned(out, dtype_size(dtype))) return NR_EINVAL;
   const int vec = 16 / dtype_size(dtype);
   if (nr_cdiv(n * ((dim + vec - 1) / vec), kThreads * kRowUnroll) > 0x7FFFFFFF) return NR_EINVAL;  // (blocks of one launch)
   const bool wide = idx_bytes == 8;
@@ -994,8 +996,8 @@ extern "C" int nr_embedding_bwd(const void* grad, int grad_dtype, int64_t grad_s
   if (!dtype_ok(grad_dtype) || !dtype_ok(table_dtype) || !sizes_ok(rows, dim, n) || (idx_bytes != 4 && idx_bytes != 8) || grad_stride < 0)
     return NR_EINVAL;
   if (rows == 0 || dim == 0) return 0;
-  if (grad_table == nullptr || (reinterpret_cast<uintptr_t>(grad_table) & (uintptr_t)(dtype_size(table_dtype) - 1)) != 0) return NR_EINVAL;
-  if (n > 0 && (grad == nullptr || idx == nullptr)) return NR_EINVAL;
+  if (grad_table == nullptr || !aligned(grad_table, dtype_size(table_dtype))) return NR_EINVAL;
+  if (n > 0 && (grad == nullptr || idx == nullptr || !aligned(grad, dtype_size(grad_dtype)) || !aligned(idx, idx_bytes))) return NR_EINVAL;
   hipStream_t st = nr_s(stream);
   SumArgs a = {};
   a.n = n;
@@ -1007,7 +1009,7 @@ extern "C" int nr_embedding_bwd(const void* grad, int grad_dtype, int64_t grad_s
   a.out_dtype = table_dtype;
   a.accumulate = accumulate;
   const OwnPlan own = n > 0 ? make_own_plan(rows, dim, n, dtype_size(grad_dtype)) : OwnPlan{};
-  if (n > 0 && own.chunks != 1 && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0)) return NR_EINVAL;
+  if (n > 0 && own.chunks != 1 && (workspace == nullptr || !aligned(workspace, 256))) return NR_EINVAL;
   if (own.chunks > 0) {
     a.group = own.group;
     a.groups = own.groups;

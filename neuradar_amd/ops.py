@@ -1319,24 +1319,20 @@ _NORM_TYPES = {2.0: 2, 1.0: 1, float("inf"): 0}
 class _GradList:
     """Addresses, sizes and types of a list of dense tensors as the host arrays that nr_grad_norm / nr_grad_scale read."""
 
-    def __init__(self, tensors: Sequence[Tensor], what: str) -> None:
-        self.count = len(tensors)
-        dtypes = [t.dtype for t in tensors]
-        if not _DTYPE_CODES.keys() >= set(dtypes):
-            raise RuntimeError(f"{what} must be float32, bfloat16 or float16")
-        devices = set(map(Tensor.get_device, tensors))
-        if len(devices) > 1 or -1 in devices:
-            raise RuntimeError(f"{what} must be GPU tensors on one device: neuradar_amd has no CPU path (the oracle is test-only)")
-        # (memory order is all that counts: a dense tensor is taken as it lies, one with holes is copied)
-        self.plain = all(map(Tensor.is_contiguous, tensors))
-        self.tensors = tensors if self.plain else [_dense(t) for t in tensors]
-        self.ptrs = array("q", map(Tensor.data_ptr, self.tensors))
-        self.numel = array("q", map(Tensor.numel, self.tensors))
-        self.dtypes = array("i", map(_DTYPE_CODES.__getitem__, dtypes))
-
-    @property
-    def arrays(self):
-        return self.ptrs.buffer_info()[0], self.numel.buffer_info()[0], self.dtypes.buffer_info()[0]
+    def __init__(self, tensors: List[Tensor], what: str) -> None:
+        self.count = n = len(tensors)
+        self.ptrs, self.numel, self.dtypes = array("q", bytes(8 * n)), array("q", bytes(8 * n)), array("i", bytes(4 * n))
+        self.arrays = self.ptrs.buffer_info()[0], self.numel.buffer_info()[0], self.dtypes.buffer_info()[0]
+        self.tensors, self.plain = tensors, True
+        self.device = _lib.tensors().nr_tensor_list(tensors, *self.arrays)
+        if self.device == -4:
+            # memory order is all that counts: a dense tensor is taken as it lies, one with holes is copied
+            self.tensors, self.plain = [_dense(t) for t in tensors], False
+            self.device = _lib.tensors().nr_tensor_list(self.tensors, *self.arrays)
+        if self.device < 0 and n > 0:
+            raise RuntimeError({-1: f"{what} must be tensors", -2: f"{what} must be float32, bfloat16 or float16",
+                                -3: f"{what} must be GPU tensors on one device: neuradar_amd has no CPU path (the oracle is test-only)"}
+                               .get(self.device, f"{what} cannot be read"))
 
 
 def _dense(t: Tensor) -> Tensor:
@@ -1351,7 +1347,7 @@ def _dense(t: Tensor) -> Tensor:
 
 
 def _norm_and_factor(lst: _GradList, max_norm: float, norm_type: float, device) -> Tensor:
-    """[norm, clip factor] on the device."""
+    """[norm, clip factor, ...] on the device."""
     kind = _NORM_TYPES.get(float(norm_type))
     if kind is None:
         raise RuntimeError(f"norm_type must be 1, 2 or infinity, not {norm_type}")
@@ -1364,7 +1360,7 @@ def _norm_and_factor(lst: _GradList, max_norm: float, norm_type: float, device) 
         raise RuntimeError("gradient list too long")
     workspace = torch.empty(2 + need // 4, device=device, dtype=torch.float32)  # [norm, factor | partial results]
     at = workspace.data_ptr()
-    check(lib.nr_grad_norm(ptrs, numel, dtypes, lst.count, kind, max_norm, at, at + 8, _launch_stream(device.index)), "nr_grad_norm")
+    check(lib.nr_grad_norm(ptrs, numel, dtypes, lst.count, kind, max_norm, at, at + 8, _launch_stream(lst.device)), "nr_grad_norm")
     return workspace
 
 
@@ -1416,6 +1412,8 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> Tens
     src = dst = _GradList(grads, "gradients")
     if out is not None:
         dst = _GradList(targets, "out")
+        if dst.device != src.device:
+            raise RuntimeError("out must be on the gradients' device")
         if dst.numel != src.numel:
             raise RuntimeError("out must hold one tensor of the same size for each gradient")
         if not (src.plain and dst.plain):  # elements are matched by place in memory: bring both into the order of their shapes
@@ -1423,15 +1421,12 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> Tens
                 raise RuntimeError("out must have its gradients' shapes where one of the two is not contiguous")
             src = _GradList([g.contiguous() for g in grads], "gradients")
             dst = _GradList([o if o.is_contiguous() else torch.empty_like(o, memory_format=torch.contiguous_format) for o in targets], "out")
-        if targets[0].device != device:
-            raise RuntimeError("out must be on the gradients' device")
-    filled = [p for p, n in zip(dst.ptrs, dst.numel) if n]
-    if len(set(filled)) != len(filled):
+    if _lib.tensors().nr_same_address(dst.arrays[0], dst.count) != 0:
         raise RuntimeError("a tensor to be written is listed twice")
     result = _norm_and_factor(src, float(max_norm), norm_type, device)
     ptrs, numel, dtypes = src.arrays
     check(_lib.lib().nr_grad_scale(ptrs, dst.arrays[0], numel, dtypes, dst.arrays[2], src.count, result.data_ptr(),
-                                   _launch_stream(device.index)), "nr_grad_scale")
+                                   _launch_stream(src.device)), "nr_grad_scale")
     if not dst.plain or dst.tensors is not targets:
         for target, written in zip(targets, dst.tensors):  # a target with holes gets its elements from a dense copy
             if written.data_ptr() != target.data_ptr():

@@ -21,12 +21,13 @@ def test_embedding_entry_points_refuse_bad_arguments():
 
     for kw in (dict(dtype=3), dict(dtype=-1), dict(rows=-1), dict(rows=0x7FFFFFFF), dict(dim=-1), dict(dim=65537), dict(idx_bytes=2), dict(n=-1),
                dict(n=0x80000000), dict(idx=None), dict(out=None), dict(table=None), dict(out_stride=7), dict(stride=-1),
-               dict(n=0x7FFFFFFF, dim=65536, out_stride=65536)):
+               dict(n=0x7FFFFFFF, dim=65536, out_stride=65536),
+               dict(idx=BIG + 4), dict(table=BIG + 2), dict(out=BIG + 1)):
         assert fwd(**kw) == E, kw
     assert fwd(n=0) == 0 and fwd(dim=0, out_stride=0) == 0
     for kw in (dict(dtype=3), dict(out_dtype=7), dict(rows=-1), dict(rows=0x7FFFFFFF), dict(dim=-1), dict(dim=65537), dict(idx_bytes=1), dict(n=-1),
                dict(n=0x80000000), dict(grad=None), dict(idx=None), dict(out=None), dict(workspace=None), dict(workspace=BIG + 8), dict(stride=-1),
-               dict(out=BIG + 2)):
+               dict(out=BIG + 2), dict(grad=BIG + 2), dict(idx=BIG + 4)):
         assert bwd(**kw) == E, kw
     assert bwd(rows=0) == 0 and bwd(dim=0) == 0 and bwd(n=0) == 0
     assert lib.nr_embedding_bwd_workspace_bytes(10, 8, -1, 0) == E and lib.nr_embedding_bwd_workspace_bytes(10, 8, 4, 5) == E
