@@ -502,6 +502,7 @@ constexpr int kOwnRangeMax = 1 << (32 - kOwnPosBits - 1);
 constexpr int kOwnBlocks = 256;
 constexpr int kOwnLanes = 32;    // half a kilobyte of a row per block at most (a kilobyte: 40 % slower where one row has a fifth of
                                  // the tokens, 64 bytes: 30 % slower where all have the same share; 4 096 rows of 1 024 in bf16)
+constexpr int64_t kOwnLateBytes = 65536;  // of zeros per block, from which on half of them wait for the sums' loads (3 us of stores)
 constexpr int kOwnSplit = 65536; // bytes of gradient that a block sums at most, on average, before a chunk is cut
 constexpr int64_t kOwnTables = (int64_t)64 << 20;  // bytes of the chunks' tables: at 78 MB as fast as the sort (260 000 tokens on
                                                    // 20 000 rows of 64 in fp32: 64 us against 74), far below it two or three times as fast
@@ -512,8 +513,22 @@ struct OwnArgs {
   SumArgs sum;
   int64_t padding;
   int range, key_bits;  // rows per block; bits of a row inside its range
+  int named_words;      // (range + 31) / 32 where a range takes long to clear, else 0
   int chunk, rounds;    // tokens per blockIdx.z, a multiple of 64; rounds of kOwnThreads that they take
 };
+
+// Zeros in rows first, first + groups, ... below `end` of the range, in this thread's columns; without those marked in `named`.
+template <int N>
+__device__ __forceinline__ void clear_rows(const SumArgs& a, const uint32_t* named, int first, int end, int64_t row0, int col) {
+  const float zero[N] = {};
+#pragma unroll 4
+  for (int q = first; q < end; q += a.groups) {
+    if (named != nullptr && ((named[q / 32] >> (q % 32)) & 1u)) continue;
+    const int64_t at = (row0 + q) * a.dim + col;
+    if (a.out_dtype == NR_DTYPE_F32) nr_store_some<float, N>(static_cast<float*>(a.out) + at, a.dim - col, zero);
+    else nr_store_some<__bf16, N>(static_cast<__bf16*>(a.out) + at, a.dim - col, zero);  // (zero is zero in both 16-bit types)
+  }
+}
 
 template <typename T, typename I>
 __global__ void __launch_bounds__(kOwnThreads)
@@ -531,7 +546,8 @@ own_kernel(OwnArgs o, const T* __restrict__ grad, const I* __restrict__ idx) {
   float* s_tail = s_head + a.groups * step;
   uint32_t* s_digit = lds;                                   // [waves][256]: before the sums
   uint32_t* s_list = lds + 2 * kOwnThreads * N;              // [chunk]
-  unsigned char* s_flag = reinterpret_cast<unsigned char*>(s_list + o.chunk);  // [groups]
+  uint32_t* s_named = s_list + o.chunk;                      // [named_words]: rows that have tokens, where they are cleared late
+  unsigned char* s_flag = reinterpret_cast<unsigned char*>(s_named + o.named_words);  // [groups]
   __shared__ uint32_t s_count[kWaves];
   __shared__ uint64_t s_span[kWaves];
   const int64_t row0 = (int64_t)blockIdx.x * o.range;
@@ -552,18 +568,18 @@ own_kernel(OwnArgs o, const T* __restrict__ grad, const I* __restrict__ idx) {
       if (d < (uint64_t)range && (uint32_t)d != padding) item[u] = ((uint32_t)d << kOwnPosBits) | (uint32_t)i;
     }
   }
-  if (!a.accumulate) {  // all rows of the range; those that are looked up are written again below, behind the barriers
+  // Zeros: the rows of the range, or of its first half, are all cleared here, beside the loads of the indices (those that are
+  // looked up are written again, behind the barriers below).  Where a range is large, the other half is cleared beside the loads
+  // of the sums, without the rows that have tokens: neither of the two latencies is left without stores (8 192 tokens on 2^22 rows of 8: 31 -> 27 us).
+  const int early = o.named_words > 0 ? range / 2 : range;
+  if (!a.accumulate) {
     if (gridDim.y == 1) {
       const int words = a.out_dtype == NR_DTYPE_F32 ? 2 : 1;
-      clear_halves(static_cast<uint16_t*>(a.out) + row0 * a.dim * words, (int64_t)range * a.dim * words, threadIdx.x, kOwnThreads);
+      clear_halves(static_cast<uint16_t*>(a.out) + row0 * a.dim * words, (int64_t)early * a.dim * words, threadIdx.x, kOwnThreads);
     } else if (work) {
-      const float zero[N] = {};
-      for (int q = r; q < range; q += a.groups) {
-        const int64_t at = (row0 + q) * a.dim + col;
-        if (a.out_dtype == NR_DTYPE_F32) nr_store_some<float, N>(static_cast<float*>(a.out) + at, a.dim - col, zero);
-        else nr_store_some<__bf16, N>(static_cast<__bf16*>(a.out) + at, a.dim - col, zero);  // (zero is zero in both 16-bit types)
-      }
+      clear_rows<N>(a, nullptr, r, early, row0, col);
     }
+    for (int w = threadIdx.x; w < o.named_words; w += kOwnThreads) s_named[w] = 0u;
   }
   uint32_t mine = 0u;
 #pragma unroll
@@ -577,7 +593,7 @@ own_kernel(OwnArgs o, const T* __restrict__ grad, const I* __restrict__ idx) {
     total += s_count[w];
   }
   const int m = (int)total;
-  if (m == 0) return;
+  if (m == 0 && (a.accumulate || o.named_words == 0)) return;
 #pragma unroll
   for (int u = 0; u < kOwnRounds; ++u) {
     if (u >= o.rounds) break;
@@ -672,6 +688,13 @@ own_kernel(OwnArgs o, const T* __restrict__ grad, const I* __restrict__ idx) {
       __syncthreads();
     }
   }
+  if (!a.accumulate && o.named_words > 0) {
+    for (int q = threadIdx.x; q < m; q += kOwnThreads) {  // (one token of each row)
+      const uint32_t key = s_list[q] >> kOwnPosBits;
+      if (q == 0 || s_list[q - 1] >> kOwnPosBits != key) atomicOr(&s_named[key / 32], 1u << (key % 32));
+    }
+    __syncthreads();
+  }
   // the sums: the groups share the list evenly, a batch of loads at least
   const int share = (m + a.groups - 1) / a.groups, per = share > kFlight ? share : kFlight;
   auto key_at = [&](int q) { return q >= 0 && q < m ? s_list[q] >> kOwnPosBits : kNone; };
@@ -684,6 +707,7 @@ own_kernel(OwnArgs o, const T* __restrict__ grad, const I* __restrict__ idx) {
       flag = walk_stretch<T, N>(a, grad, q0, q1, col, (uint32_t)row0, key_at,
                                 [&](int q) { return s_list[q] & ((1u << kOwnPosBits) - 1u); }, head, tail);
     if (glane == 0) s_flag[r] = (unsigned char)flag;
+    if (!a.accumulate && o.named_words > 0) clear_rows<N>(a, s_named, early + r, range, row0, col);
   }
   __syncthreads();
   mark_spans(s_flag, a.groups, s_span);
@@ -932,13 +956,15 @@ int launch_sum(const Plan& p, const SumArgs& a, const void* grad, hipStream_t st
   return 0;
 }
 
-constexpr size_t own_lds(int vec, int list_words) { return (size_t)(2 * kOwnThreads * vec + list_words) * 4 + kOwnThreads; }
+constexpr size_t own_lds(int vec, int list_words, int named_words) {
+  return (size_t)(2 * kOwnThreads * vec + list_words + named_words) * 4 + kOwnThreads;
+}
 
 template <typename T, typename I>
 int launch_own(const OwnPlan& p, const OwnArgs& o, const void* grad, const void* idx, hipStream_t stream) {
   constexpr int N = 16 / (int)sizeof(T);
   hipLaunchKernelGGL((own_kernel<T, I>), dim3((uint32_t)p.ranges, (uint32_t)p.col_tiles, (uint32_t)p.chunks), dim3(kOwnThreads),
-                     own_lds(N, o.chunk), stream, o, static_cast<const T*>(grad), static_cast<const I*>(idx));
+                     own_lds(N, o.chunk, o.named_words), stream, o, static_cast<const T*>(grad), static_cast<const I*>(idx));
   NR_LAUNCH_CHECK();
   return 0;
 }
@@ -946,8 +972,8 @@ int launch_own(const OwnPlan& p, const OwnArgs& o, const void* grad, const void*
 template <typename T>
 int init_own() {
   constexpr int N = 16 / (int)sizeof(T);
-  if (int rc = nr_raise_lds(own_kernel<T, int64_t>, own_lds(N, kOwnMax))) return rc;
-  return nr_raise_lds(own_kernel<T, int32_t>, own_lds(N, kOwnMax));
+  if (int rc = nr_raise_lds(own_kernel<T, int64_t>, own_lds(N, kOwnMax, kOwnRangeMax / 32))) return rc;
+  return nr_raise_lds(own_kernel<T, int32_t>, own_lds(N, kOwnMax, kOwnRangeMax / 32));
 }
 
 template <typename O>
@@ -1019,7 +1045,8 @@ extern "C" int nr_embedding_bwd(const void* grad, int grad_dtype, int64_t grad_s
       a.accumulate = 0;
       a.scale = 1.0f;
     }
-    const OwnArgs o = {a, padding, own.range, own.key_bits, own.chunk, (own.chunk + kOwnThreads - 1) / kOwnThreads};
+    const int named = own.col_tiles == 1 && (int64_t)own.range * dim * (int64_t)sizeof(float) >= kOwnLateBytes ? (own.range + 31) / 32 : 0;
+    const OwnArgs o = {a, padding, own.range, own.key_bits, named, own.chunk, (own.chunk + kOwnThreads - 1) / kOwnThreads};
     const bool wide = idx_bytes == 8;
     auto launch = grad_dtype == NR_DTYPE_F32    ? (wide ? launch_own<float, int64_t> : launch_own<float, int32_t>)
                   : grad_dtype == NR_DTYPE_BF16 ? (wide ? launch_own<__bf16, int64_t> : launch_own<__bf16, int32_t>)

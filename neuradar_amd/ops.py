@@ -701,6 +701,7 @@ def radar_loss(pred: Tensor, detections: Tensor, seg: Tensor, max_detections: in
 # ------------------------------------------------------------------------------------------------ embedding rows
 _DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # NR_DTYPE_*
 _raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream of a device as an address, without a Stream object
+_current_device = torch._C._cuda_getDevice  # (behind a tensor on a device: initialised)
 
 
 def _launch_stream(device: int) -> int:
@@ -745,7 +746,7 @@ def _strided_rows(t: Tensor) -> Tuple[Tensor, int]:
 
 def _embedding_rows(table: Tensor, idx: Tensor, scale: float) -> Tensor:
     device = table.get_device()
-    if device != torch.cuda.current_device():
+    if device != _current_device():
         with torch.cuda.device(device):
             return _embedding_rows(table, idx, scale)
     rows, dim = table.shape
@@ -764,7 +765,7 @@ def embedding_grad(grad: Tensor, idx: Tensor, num_rows: int, scale: float = 1.0,
     out: contiguous [num_rows, dim] that takes the result; accumulate: added to what `out` holds (rows that no index names are not
     touched).  Indices equal to padding_idx or outside [0, num_rows) contribute nothing."""
     device = grad.get_device()
-    if device >= 0 and device != torch.cuda.current_device():
+    if device >= 0 and device != _current_device():
         with torch.cuda.device(device):
             return embedding_grad(grad, idx, num_rows, scale, padding_idx, out, accumulate, dtype)
     if grad.dim() != idx.dim() + 1 or grad.shape[:-1] != idx.shape:
@@ -1375,7 +1376,7 @@ def grad_norm(grads, norm_type: float = 2.0) -> Tensor:
     if not grads:
         return torch.zeros((), device="cuda", dtype=torch.float32)
     device = grads[0].device
-    if device.type == "cuda" and device.index != torch.cuda.current_device():
+    if device.type == "cuda" and device.index != _current_device():
         with torch.cuda.device(device):
             return grad_norm(grads, norm_type)
     return _norm_and_factor(_GradList(grads, "gradients"), float("inf"), norm_type, device)[0]
@@ -1388,7 +1389,7 @@ def clip_factor(grads, max_norm: float, norm_type: float = 2.0) -> Tuple[Tensor,
     if not grads:
         raise RuntimeError("clip_factor: no gradients")
     device = grads[0].device
-    if device.type == "cuda" and device.index != torch.cuda.current_device():
+    if device.type == "cuda" and device.index != _current_device():
         with torch.cuda.device(device):
             return clip_factor(grads, max_norm, norm_type)
     result = _norm_and_factor(_GradList(grads, "gradients"), float(max_norm), norm_type, device)
@@ -1406,7 +1407,7 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> Tens
     if not grads:
         return torch.zeros((), device="cuda", dtype=torch.float32)
     device = grads[0].device
-    if device.type == "cuda" and device.index != torch.cuda.current_device():
+    if device.type == "cuda" and device.index != _current_device():
         with torch.cuda.device(device):
             return clip_grads(grads, max_norm, norm_type, out)
     src = dst = _GradList(grads, "gradients")
