@@ -507,7 +507,7 @@ constexpr int kOwnSplit = 65536; // bytes of gradient that a block sums at most,
 constexpr int64_t kOwnTables = (int64_t)64 << 20;  // bytes of the chunks' tables: at 78 MB as fast as the sort (260 000 tokens on
                                                    // 20 000 rows of 64 in fp32: 64 us against 74), far below it two or three times as fast
 constexpr int kCountSort = 256;  // lists up to this length: every entry counts the smaller ones
-constexpr int kOwnDigitBits = 8;
+constexpr int kOwnDigitBits = 9;  // (32 KB of counters)
 
 struct OwnArgs {
   SumArgs sum;
@@ -544,7 +544,7 @@ own_kernel(OwnArgs o, const T* __restrict__ grad, const I* __restrict__ idx) {
   const int step = a.group * N, lane = nr_lane(), wave = threadIdx.x / NR_WAVE;
   float* s_head = reinterpret_cast<float*>(lds);             // [groups][group * N]
   float* s_tail = s_head + a.groups * step;
-  uint32_t* s_digit = lds;                                   // [waves][256]: before the sums
+  uint32_t* s_digit = lds;                                   // [waves][512]: before the sums
   uint32_t* s_list = lds + 2 * kOwnThreads * N;              // [chunk]
   uint32_t* s_named = s_list + o.chunk;                      // [named_words]: rows that have tokens, where they are cleared late
   unsigned char* s_flag = reinterpret_cast<unsigned char*>(s_named + o.named_words);  // [groups]
@@ -614,7 +614,7 @@ own_kernel(OwnArgs o, const T* __restrict__ grad, const I* __restrict__ idx) {
     if ((int)threadIdx.x < m) s_list[place] = own;
     __syncthreads();
   } else if (range > 1) {
-    // by 8 bits of the row at a time, as in sort_scatter_kernel: the list through registers and back
+    // by 9 bits of the row at a time, as in sort_scatter_kernel: the list through registers and back
     const int rounds = (m + kOwnThreads - 1) / kOwnThreads;
     for (int shift = 0; shift < o.key_bits; shift += kOwnDigitBits) {
       constexpr int kDigits = 1 << kOwnDigitBits;
@@ -645,7 +645,7 @@ own_kernel(OwnArgs o, const T* __restrict__ grad, const I* __restrict__ idx) {
         rank[u] = old + (uint32_t)__popcll(peers & ((1ull << lane) - 1ull));
       }
       __syncthreads();
-      // exclusive prefix over (digit, wave): a thread per digit adds its waves, the first wave scans the 256 sums
+      // exclusive prefix over (digit, wave): a thread per digit adds its waves, the first wave scans the sums
       __shared__ uint32_t s_first[kDigits];
       if (threadIdx.x < kDigits) {
         uint32_t sum = 0u;
@@ -659,10 +659,11 @@ own_kernel(OwnArgs o, const T* __restrict__ grad, const I* __restrict__ idx) {
       }
       __syncthreads();
       if (wave == 0) {
-        uint32_t c[4], sum = 0u;
+        constexpr int kPer = kDigits / NR_WAVE;
+        uint32_t c[kPer], sum = 0u;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          c[k] = s_first[lane * 4 + k];
+        for (int k = 0; k < kPer; ++k) {
+          c[k] = s_first[lane * kPer + k];
           sum += c[k];
         }
         uint32_t incl = sum;
@@ -673,8 +674,8 @@ own_kernel(OwnArgs o, const T* __restrict__ grad, const I* __restrict__ idx) {
         }
         uint32_t run = incl - sum;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          s_first[lane * 4 + k] = run;
+        for (int k = 0; k < kPer; ++k) {
+          s_first[lane * kPer + k] = run;
           run += c[k];
         }
       }
