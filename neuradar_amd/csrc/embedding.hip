@@ -500,6 +500,7 @@ constexpr int kOwnMax = kOwnThreads * kOwnRounds;  // 14 bits of position, 18 of
 constexpr int kOwnPosBits = 14;
 constexpr int kOwnRangeMax = 1 << (32 - kOwnPosBits - 1);
 constexpr int kOwnBlocks = 256;
+constexpr int kOwnChunkMin = 2048;
 constexpr int kOwnLanes = 32;    // half a kilobyte of a row per block at most (a kilobyte: 40 % slower where one row has a fifth of
                                  // the tokens, 64 bytes: 30 % slower where all have the same share; 4 096 rows of 1 024 in bf16)
 constexpr int64_t kOwnLateBytes = 65536;  // of zeros per block, from which on half of them wait for the sums' loads (3 us of stores)
@@ -867,30 +868,37 @@ OwnPlan make_own_plan(int64_t rows, int dim, int64_t n, int elem_size) {
   OwnPlan p = {};
   if (rows > (int64_t)kOwnRangeMax * kOwnBlocks) return p;  // (18 bits of a list entry for the row)
   const int vec = 16 / elem_size, nv = (dim + vec - 1) / vec;
-  auto cut = [&](int chunk) {
-    p.chunk = chunk;
-    p.chunks = (int)nr_cdiv(n, chunk);
-    const int blocks = p.chunks < kOwnBlocks ? (kOwnBlocks + p.chunks - 1) / p.chunks : 1;
-    int lanes = nv < kOwnLanes ? nv : kOwnLanes;  // half a kilobyte of a row, then down to 64 bytes while there are CUs without a block
-    while (lanes > 4 && rows * ((nv + lanes - 1) / lanes) < blocks) lanes = (lanes + 1) / 2;
+  const int64_t least = nr_cdiv(n, kOwnMax), most = nr_cdiv(n, kOwnChunkMin);
+  // at most kOwnBlocks blocks, one to a CU: more would wait for the first to end (113 840 tokens on 1 999 rows: 259 blocks 26 to 32 us,
+  // 252 blocks 24 us)
+  auto cut = [&](int64_t chunks, int lanes) {
+    p.chunk = (int)(nr_cdiv(nr_cdiv(n, chunks), NR_WAVE) * NR_WAVE);
+    p.chunks = (int)nr_cdiv(n, p.chunk);
     p.col_tiles = (nv + lanes - 1) / lanes;
-    const int64_t want = p.col_tiles < blocks ? (blocks + p.col_tiles - 1) / p.col_tiles : 1;
-    int64_t range = nr_cdiv(rows, want);
+    const int64_t want = kOwnBlocks / ((int64_t)p.col_tiles * p.chunks);
+    int64_t range = nr_cdiv(rows, want > 0 ? want : 1);
     if (range > kOwnRangeMax) range = kOwnRangeMax;
     p.range = (int)range;
     p.ranges = (int)nr_cdiv(rows, range);
   };
-  cut(n < kOwnMax ? (int)(nr_cdiv(n, NR_WAVE) * NR_WAVE) : kOwnMax);
-  // few rows, or wide ones: their tokens on more blocks.  (In one chunk only where a block has much to read: a second launch
-  // costs 3 us.  16 384 tokens on one row of 1 024: 56 -> 34 us)
-  auto per_block = [&] { return nr_cdiv(p.chunk, p.ranges) * nr_cdiv(nv, p.col_tiles) * 16; };
-  if (p.chunks > 1 || per_block() > kOwnSplit)
-    while (p.chunk > 2048 && p.ranges * p.col_tiles * p.chunks < kOwnBlocks) cut(p.chunk > 4096 ? p.chunk / 128 * 64 : 2048);
-  if (p.chunks > 1 && (double)p.chunks * (double)rows * dim * sizeof(float) > (double)kOwnTables) {
-    if (n <= kOwnMax) cut((int)(nr_cdiv(n, NR_WAVE) * NR_WAVE));  // (one chunk needs no tables)
-    else p.chunks = 0;
+  auto blocks = [&] { return (int64_t)p.ranges * p.col_tiles * p.chunks; };
+  int lanes = nv < kOwnLanes ? nv : kOwnLanes;  // half a kilobyte of a row, then down to 64 bytes while there are CUs without a block
+  if (least == 1) {
+    while (lanes > 4 && rows * ((nv + lanes - 1) / lanes) < kOwnBlocks) lanes = (lanes + 1) / 2;
+    cut(1, lanes);
+    // (a second launch costs 3 us: only for blocks with much to read.  16 384 tokens on one row of 1 024: 56 -> 34 us)
+    if (blocks() <= kOwnBlocks / 2 && nr_cdiv(n, p.ranges) * nr_cdiv(nv, p.col_tiles) * 16 > kOwnSplit) {
+      const int64_t more = kOwnBlocks / blocks();
+      cut(more < most ? more : most, lanes);
+      if (p.chunks > 1 && (double)p.chunks * (double)rows * dim * sizeof(float) > (double)kOwnTables) cut(1, lanes);
+    }
+  } else {
+    cut(least, lanes);
+    const int64_t more = kOwnBlocks / ((int64_t)p.ranges * p.col_tiles);
+    if (more > least) cut(more < most ? more : most, lanes);
+    while (lanes > 4 && blocks() <= kOwnBlocks / 2) cut(p.chunks, lanes = (lanes + 1) / 2);
+    if (p.chunks > 65535 || (double)p.chunks * (double)rows * dim * sizeof(float) > (double)kOwnTables) p.chunks = 0;
   }
-  if (p.chunks > 65535) p.chunks = 0;
   p.group = (nv + p.col_tiles - 1) / p.col_tiles;
   p.groups = kOwnThreads / p.group;
   while (((p.range - 1) >> p.key_bits) != 0) ++p.key_bits;
