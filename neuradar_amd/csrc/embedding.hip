@@ -505,8 +505,9 @@ constexpr int kOwnLanes = 32;    // half a kilobyte of a row per block at most (
                                  // the tokens, 64 bytes: 30 % slower where all have the same share; 4 096 rows of 1 024 in bf16)
 constexpr int64_t kOwnLateBytes = 65536;  // of zeros per block, from which on half of them wait for the sums' loads (3 us of stores)
 constexpr int kOwnSplit = 65536; // bytes of gradient that a block sums at most, on average, before a chunk is cut
-constexpr int64_t kOwnTables = (int64_t)64 << 20;  // bytes of the chunks' tables: at 78 MB as fast as the sort (260 000 tokens on
-                                                   // 20 000 rows of 64 in fp32: 64 us against 74), far below it two or three times as fast
+constexpr int64_t kOwnTables = (int64_t)64 << 20;  // bytes of the chunks' tables.  26 MB: 27 us against 41 sorted (40 000 tokens
+                                                   // on 30 000 rows of 64 in fp32), 78 MB: 57 against 75, 156 MB: 78 against 76; in
+                                                   // bf16 the sort's own traffic is half of that, 128 MB: 58 against 44
 constexpr int kCountSort = 256;  // lists up to this length: every entry counts the smaller ones
 constexpr int kOwnDigitBits = 9;  // (32 KB of counters)
 
@@ -845,7 +846,8 @@ Plan make_plan(int64_t rows, int dim, int64_t n, int elem_size) {
   p.groups = kThreads / p.group;
   p.per_group = 64;
   while (p.groups * p.per_group > kMaxStretch) p.per_group /= 2;
-  while (p.per_group > kFlight && nr_cdiv(n, (int64_t)p.groups * p.per_group) * p.col_tiles < 1024) p.per_group /= 2;
+  // (three blocks to a CU: 100 000 x 512 bf16 61 us against 73 with four, 131 072 x 512 91 against 104 with two)
+  while (p.per_group > kFlight && nr_cdiv(n, (int64_t)p.groups * p.per_group) * p.col_tiles < 3 * kOwnBlocks) p.per_group /= 2;
   p.sum_blocks = (uint32_t)nr_cdiv(n, (int64_t)p.groups * p.per_group);
   auto place = [&p](int64_t bytes) {
     const int64_t at = p.bytes;
