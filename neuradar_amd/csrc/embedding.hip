@@ -4,17 +4,23 @@
 //   gradient  g_table[v, :] (+)= round(scale * sum over i with idx[i] = v of g[i, :])         (nr_embedding_bwd)
 //
 // The gradient is a sum over equal indices.  Adding rows to the table as they come needs float atomics, whose order -- and with
-// it the result -- changes from run to run, and a row that many tokens share becomes one queue at the memory side.  Here the
-// (index, position) pairs are SORTED first (stable, so equal indices keep their positions in ascending order); then equal
-// indices are neighbours, every sum is formed in registers in one fixed order, and each touched row is written once.
-//   * sort: least significant digit first, digits of up to 11 bits (one pass for 2 047 rows, two for 4 M); per pass a count, a
-//     scan and a scatter.  Indices that get no gradient (padding, out of range) take the key `rows` and end up last.
-//   * sum: a block takes a fixed stretch of SORTED positions, whatever the indices are -- a row that owns half of the batch is
-//     spread over as many blocks as its tokens need.  Groups of lanes walk shorter stretches, U rows of g in flight each; a sum
-//     whose neighbours lie in other stretches goes through LDS to its first group, one that leaves the block is left in the
-//     workspace.
-//   * join: sums that cross blocks are added up in block order by the block they start in.
-// All sums are held in fp32; the order is that of the stretches, fixed by (n, dim) alone: two calls give the same bits.
+// it the result -- changes from run to run, and a row that many tokens share becomes one queue at the memory side.  Here equal
+// indices are brought together first, their positions in ascending order; then every sum is formed in registers in one fixed
+// order and each touched row is written once.  All sums are held in fp32; the order follows from (n, rows, dim, type) alone: two
+// calls give the same bits.  Three ways, by sizes (make_own_plan, make_plan):
+//   * up to 16 384 indices, one launch: a block owns a range of rows, picks its tokens out of all indices and orders them in LDS
+//     (own_kernel);
+//   * more indices and a table whose copies are small: the same on chunks of the indices, and a launch that adds the chunks' tables;
+//   * else: (index, position) pairs are sorted, least significant digit first, digits of up to 11 bits (one pass for 2 047 rows,
+//     two for 4 M), a count, a scan and a scatter per pass.  A block sums a fixed stretch of SORTED positions, whatever the
+//     indices are -- a row that owns half of the batch is spread over as many blocks as its tokens need.  Groups of lanes walk
+//     shorter stretches, 8 rows of g in flight each; a sum whose neighbours lie in other stretches goes through LDS to its first
+//     group, one that leaves the block is left in the workspace and added up in block order by a last launch.
+// Bound by memory where rows are long (read g once, write the table once), by the chain of launches and of dependent steps inside
+// a block where they are few.  Measured, kernels alone: rows 262 144 x 1 024 bf16 114 us (0.69 GB of traffic: 6.0 TB/s; 153 us on
+// a cold table); gradient 16 384 x 16 on 60 rows 12 us, 113 840 x 32 on 1 999 rows 21 + 4, 8 192 x 8 on 2^22 rows 27 (134 MB of
+// zeros alone: 18), 100 003 x 257 on 7 rows 34 + 5 (103 MB: 20), 131 072 x 512 bf16 on 131 072 rows 108 (sort 45, which also
+// writes the zeros; sums 53 at 3.2 TB/s; join 9).
 #include "rows_dev.h"
 
 namespace {
