@@ -783,6 +783,8 @@ def embedding_grad(grad: Tensor, idx: Tensor, num_rows: int, scale: float = 1.0,
     elif (_float_rows(out, "out").shape != (num_rows, dim) or not out.is_contiguous() or out.get_device() != device
           or dtype not in (None, out.dtype)):
         raise RuntimeError(f"out must be a contiguous [{num_rows}, {dim}] tensor on grad's device" + ("" if dtype is None else f" of {dtype}"))
+    if n > 0 and dim > 0 and out.data_ptr() == grad.data_ptr():
+        raise RuntimeError("out must not be grad")
     grad, stride = _strided_rows(grad)
     code = _DTYPE_CODES[grad.dtype]
     lib = _lib.lib()
@@ -790,7 +792,7 @@ def embedding_grad(grad: Tensor, idx: Tensor, num_rows: int, scale: float = 1.0,
     if need < 0:
         raise RuntimeError(f"embedding_grad: sizes out of range ({n} indices, {num_rows} rows of {dim})")
     workspace = grad.new_empty(need, dtype=torch.uint8) if need else None
-    check(lib.nr_embedding_bwd(grad.data_ptr(), code, stride, idx.data_ptr(), idx.element_size(), n, num_rows, dim, scale, padding,
+    check(lib.nr_embedding_bwd(grad.data_ptr(), code, stride, idx.data_ptr(), idx.element_size(), n, num_rows, dim, float(scale), padding,
                                out.data_ptr(), _DTYPE_CODES[out.dtype], accumulate, None if workspace is None else workspace.data_ptr(),
                                _launch_stream(device)), "nr_embedding_bwd")
     return out
@@ -1398,8 +1400,9 @@ def clip_factor(grads, max_norm: float, norm_type: float = 2.0) -> Tuple[Tensor,
 
 def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> Tensor:
     """Scale gradients by min(1, max_norm / (norm + 1e-6)), norm = grad_norm(grads, norm_type), which is returned.  In place, or
-    into the tensors of `out` (as many elements each, any of the three types: places in a 16-bit bucket, say), one rounding.  Nothing is read on
-    the host; a norm of NaN makes every gradient NaN, as in torch."""
+    into the tensors of `out` (as many elements each, any of the three types: places in a 16-bit bucket, say), one rounding.
+    Nothing is read on the host; a norm of NaN makes every gradient NaN, as in torch.  Tensors that are written must not share
+    memory (two that start at one address are refused)."""
     grads = _as_list(grads)
     targets = grads if out is None else _as_list(out)
     if len(targets) != len(grads):
@@ -1409,7 +1412,7 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> Tens
     device = grads[0].device
     if device.type == "cuda" and device.index != _current_device():
         with torch.cuda.device(device):
-            return clip_grads(grads, max_norm, norm_type, out)
+            return clip_grads(grads, max_norm, norm_type, None if out is None else targets)
     src = dst = _GradList(grads, "gradients")
     if out is not None:
         dst = _GradList(targets, "out")

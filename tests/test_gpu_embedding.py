@@ -228,6 +228,50 @@ def test_refusals():
                        (lambda: ops.embedding_grad(g, idx, 4, out=table[:3]), "contiguous"), (lambda: ops.embedding_grad(g, idx, 4, dtype=torch.float64), "dtype"),
                        (lambda: ops.embedding_grad(g, idx, 4, out=torch.zeros(4, 4, device=DEV)[:, :2]), "contiguous"),
                        (lambda: ops.embedding_grad(g, idx, 4, out=table, dtype=BF16), "contiguous"), (lambda: ops.embedding_grad(g, idx, 4, padding_idx=9), "not a row"),
-                       (lambda: ops.embedding_grad(g, idx, 2 ** 31), "out of range"), (lambda: ops.embedding_grad(g[:2], idx, 4), "does not fit")):
+                       (lambda: ops.embedding_grad(g, idx, 2 ** 31), "out of range"), (lambda: ops.embedding_grad(g, idx, 3, out=g), "must not be grad"), (lambda: ops.embedding_grad(g[:2], idx, 4), "does not fit")):
         with pytest.raises(RuntimeError, match=what):
             call()
+
+
+def test_far_offsets():
+    """Tables and gradients of more than 2^31 elements: every offset in 64 bits, in each of the three ways to the gradient."""
+    rows, dim = 2_200_000, 1024
+    table = torch.zeros(rows, dim, device=DEV, dtype=BF16)
+    idx = torch.tensor([rows - 1, 0, rows - 2, rows - 1], device=DEV)
+    table[-2:] = torch.randn(2, dim, device=DEV).to(BF16)
+    assert torch.equal(ops.embedding(table, idx), table[idx])
+    g = torch.randn(4, dim, device=DEV).to(BF16)
+    out = ops.embedding_grad(g, idx, rows, out=table)  # one launch
+    assert torch.equal(out[-2], g[2]) and torch.equal(out[0], g[1]) and float(out[1:-2].abs().max()) == 0.0
+    assert torch.equal(out[-1], (g[0].float() + g[3].float()).to(BF16))
+    many = torch.full((20000,), rows - 1, device=DEV)
+    many[::2] = rows - 2
+    ones = torch.ones(1, dim, device=DEV, dtype=BF16).expand(20000, dim)
+    out = ops.embedding_grad(ones, many, rows, out=table)  # sorted: the tables of two chunks would not be small
+    assert bool((out[-2:] == torch.tensor(10000.0, device=DEV).to(BF16)).all()) and float(out[:-2].abs().max()) == 0.0
+    del out, table
+    grad = torch.zeros(rows, dim, device=DEV, dtype=BF16)
+    grad[-3:] = 1.0
+    got = ops.embedding_grad(grad, torch.arange(rows, device=DEV) % 7, 7)  # chunks into small tables
+    want = torch.zeros(7, dim, device=DEV, dtype=BF16)
+    want[[(rows - k) % 7 for k in (1, 2, 3)]] = 1.0
+    assert torch.equal(got, want)
+
+
+def test_two_streams_at_once_and_no_second_derivative():
+    sets = []
+    for k, (n, rows, dim) in enumerate(((3000, 40, 16), (30000, 900, 24), (30000, 700000, 40))):
+        sets.append((torch.randn(n, dim, device=DEV), indices(n, rows, "skewed", k).to(DEV), rows))
+    alone = [ops.embedding_grad(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = []
+    for s, st in zip(sets, streams):
+        with torch.cuda.stream(st):
+            got.append([ops.embedding_grad(*s) for _ in range(5)])
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, bs in zip(alone, got) for b in bs)
+    table = torch.randn(5, 3, device=DEV, requires_grad=True)
+    (first,) = torch.autograd.grad(ops.embedding(table, torch.tensor([1, 2], device=DEV)).square().sum(), table, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable|does not require grad|differentiable"):
+        first.sum().backward()
