@@ -567,13 +567,18 @@ own_kernel(OwnArgs o, const T* __restrict__ grad, const I* __restrict__ idx) {
   uint32_t item[kOwnRounds];
   constexpr uint32_t kNone = 0xFFFFFFFFu;
   const uint32_t padding = o.padding >= row0 && o.padding < row0 + range ? (uint32_t)(o.padding - row0) : kNone;
+  const int first = wave * (NR_WAVE * o.rounds) + lane;
+  I raw[kOwnRounds];  // (all loads before the first test: past the end the last index again)
+#pragma unroll
+  for (int u = 0; u < kOwnRounds; ++u)
+    if (u < o.rounds) raw[u] = idx[first + u * NR_WAVE < n ? first + u * NR_WAVE : n - 1];
 #pragma unroll
   for (int u = 0; u < kOwnRounds; ++u) {
     item[u] = kNone;
-    const int i = wave * (NR_WAVE * o.rounds) + u * NR_WAVE + lane;
-    if (u < o.rounds && i < n) {
-      const uint64_t d = (uint64_t)((int64_t)idx[i] - row0);  // (below the range: far above it)
-      if (d < (uint64_t)range && (uint32_t)d != padding) item[u] = ((uint32_t)d << kOwnPosBits) | (uint32_t)i;
+    const int i = first + u * NR_WAVE;
+    if (u < o.rounds) {
+      const uint64_t d = (uint64_t)((int64_t)raw[u] - row0);  // (below the range: far above it)
+      if (i < n && d < (uint64_t)range && (uint32_t)d != padding) item[u] = ((uint32_t)d << kOwnPosBits) | (uint32_t)i;
     }
   }
   // Zeros: the rows of the range, or of its first half, are all cleared here, beside the loads of the indices (those that are
@@ -606,6 +611,7 @@ own_kernel(OwnArgs o, const T* __restrict__ grad, const I* __restrict__ idx) {
   for (int u = 0; u < kOwnRounds; ++u) {
     if (u >= o.rounds) break;
     const uint64_t hit = __ballot(item[u] != kNone);
+    if (hit == 0ull) continue;
     if (item[u] != kNone) s_list[at + (uint32_t)__popcll(hit & ((1ull << lane) - 1ull))] = item[u];
     at += (uint32_t)__popcll(hit);
   }
