@@ -981,6 +981,7 @@ int nr_adam_hyper(float* step_t, float* dev_hyper, float lr, float lr_final, int
  *                   order; result[1] = min(1, max_norm / (result[0] + 1e-6)), NaN if the norm is.  max_norm >= 0 (infinity: a
  *                   factor of 1).  NaN and infinities of the gradients reach the norm.  No elements: norm 0.
  *   nr_grad_scale   outs[t] = round(result[1] * grads[t]); outs[t] == grads[t] is in place, and then a factor of 1 moves nothing
+ *   nr_grad_clip    nr_grad_norm and nr_grad_scale in one call (the same results; one launch less for short lists)
  *   workspace       nr_grad_norm_workspace_bytes(numel, count) bytes, 8-byte aligned
  * nr_adam_step_clipped: nr_adam_step with the gradient multiplied by clip[0] (device float; result + 1 of nr_grad_norm) besides
  * grad_scale -- clipping inside the optimizer's own pass, the gradients are not rewritten for it.
@@ -990,6 +991,9 @@ int nr_grad_norm(const void* const* grads, const int64_t* numel, const int32_t* 
                  float* result, void* workspace, nr_stream_t stream);
 int nr_grad_scale(const void* const* grads, void* const* outs, const int64_t* numel, const int32_t* dtypes,
                   const int32_t* out_dtypes, int count, const float* result, nr_stream_t stream);
+int nr_grad_clip(const void* const* grads, void* const* outs, const int64_t* numel, const int32_t* dtypes,
+                 const int32_t* out_dtypes, int count, int norm_type, double max_norm, float* result, void* workspace,
+                 nr_stream_t stream);
 int nr_adam_step_clipped(float* param, float* grad, float* exp_avg, float* exp_avg_sq, int64_t n,
                          float lr, float beta1, float beta2, float eps, float weight_decay, int adamw,
                          int step, float grad_scale, int zero_grad, const float* dev_hyper, uint8_t* seen_grad,

@@ -188,6 +188,7 @@ PROTOTYPES = {
     "nr_grad_norm_workspace_bytes": [P, I],
     "nr_grad_norm": [P, P, P, I, I, D, P, P, P],
     "nr_grad_scale": [P, P, P, P, P, I, P, P],
+    "nr_grad_clip": [P, P, P, P, P, I, I, D, P, P, P],
     "nr_adam_step_clipped": [P, P, P, P, L, F, F, F, F, F, I, I, F, I, P, P, P, P, I, P, P],
     "nr_apply_delta16": [P, P, L, L, L, P],
     "nr_grad_to16_clear": [P, P, L, P],

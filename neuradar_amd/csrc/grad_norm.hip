@@ -21,6 +21,7 @@ constexpr int kUnroll = 4;                   // 16-byte accesses in flight per t
 constexpr int kPiece = kThreads * kUnroll * 8;  // elements: pieces of whole batches for 16-bit and 32-bit types
 constexpr int64_t kMaxBlocks = 16384;        // pieces that a list is cut into, about
 constexpr int kFinishThreads = 1024;
+constexpr int64_t kFew = 1024;               // partial results that a block adds up beside other work
 
 enum { kNormMax = 0, kNormSum = 1, kNormTwo = 2 };
 
@@ -128,24 +129,33 @@ norm_kernel(List l, double* __restrict__ partial) {
   if (threadIdx.x == 0) partial[blockIdx.x] = v;
 }
 
-// result[0] = norm, result[1] = the factor that clips to max_norm
-template <int KIND>
-__global__ void __launch_bounds__(kFinishThreads)
-norm_finish_kernel(const double* __restrict__ partial, int64_t count, double max_norm, float* __restrict__ result) {
+// The partial results' norm, and the factor that clips to max_norm, in thread 0 of the block.
+template <int KIND, int THREADS>
+__device__ __forceinline__ void finish(const double* __restrict__ partial, int64_t count, double max_norm, float& norm, float& factor) {
   Acc<KIND> acc;
-  for (int64_t i = threadIdx.x; i < count; i += 4 * kFinishThreads) {
+  for (int64_t i = threadIdx.x; i < count; i += 4 * THREADS) {
     double v[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) v[u] = i + u * kFinishThreads < count ? partial[i + u * kFinishThreads] : 0.0;
+    for (int u = 0; u < 4; ++u) v[u] = i + u * THREADS < count ? partial[i + u * THREADS] : 0.0;
 #pragma unroll
     for (int u = 0; u < 4; ++u) acc.join(v[u]);
   }
-  double v = block_reduce<KIND, kFinishThreads>(acc);
+  double v = block_reduce<KIND, THREADS>(acc);
+  if constexpr (KIND == kNormTwo) v = sqrt(v);
+  const double f = max_norm / (v + 1e-6);
+  norm = (float)v;
+  factor = f > 1.0 ? 1.0f : (float)f;  // (NaN stays NaN)
+}
+
+// result[0] = norm, result[1] = factor
+template <int KIND, int THREADS>
+__global__ void __launch_bounds__(THREADS)
+norm_finish_kernel(const double* __restrict__ partial, int64_t count, double max_norm, float* __restrict__ result) {
+  float norm, factor;
+  finish<KIND, THREADS>(partial, count, max_norm, norm, factor);
   if (threadIdx.x == 0) {
-    if constexpr (KIND == kNormTwo) v = sqrt(v);
-    const double f = max_norm / (v + 1e-6);
-    result[0] = (float)v;
-    result[1] = f > 1.0 ? 1.0f : (float)f;  // (NaN stays NaN)
+    result[0] = norm;
+    result[1] = factor;
   }
 }
 
@@ -182,11 +192,7 @@ __device__ __forceinline__ void piece_scale_to(const T* x, void* y, int out_dtyp
 }
 
 template <bool STREAM>
-__global__ void __launch_bounds__(kThreads)
-scale_kernel(List l, const float* __restrict__ result) {
-  const float f = result[1];
-  // backwards: what the norm read last is what the cache still holds
-  const uint32_t block = gridDim.x - 1 - blockIdx.x;
+__device__ __forceinline__ void scale_block(const List& l, uint32_t block, float f) {
   const int t = tensor_of(l, block);
   if (f == 1.0f && l.in[t] == l.out[t]) return;  // in place and within the norm: nothing to do
   const int64_t lo = (int64_t)(block - l.first[t]) * l.piece;
@@ -194,6 +200,32 @@ scale_kernel(List l, const float* __restrict__ result) {
   if (l.in_dtype[t] == NR_DTYPE_F32) piece_scale_to<float, STREAM>(static_cast<const float*>(l.in[t]), l.out[t], l.out_dtype[t], lo, hi, f);
   else if (l.in_dtype[t] == NR_DTYPE_BF16) piece_scale_to<__bf16, STREAM>(static_cast<const __bf16*>(l.in[t]), l.out[t], l.out_dtype[t], lo, hi, f);
   else piece_scale_to<_Float16, STREAM>(static_cast<const _Float16*>(l.in[t]), l.out[t], l.out_dtype[t], lo, hi, f);
+}
+
+template <bool STREAM>
+__global__ void __launch_bounds__(kThreads)
+scale_kernel(List l, const float* __restrict__ result) {
+  // backwards: what the norm read last is what the cache still holds
+  scale_block<STREAM>(l, gridDim.x - 1 - blockIdx.x, result[1]);
+}
+
+// The same straight from the partial results, where they are few: every block adds them up for itself, in the finishing launch's
+// order, and that launch (3 us with the wait for it) is saved.
+template <int KIND>
+__global__ void __launch_bounds__(kThreads)
+finish_scale_kernel(List l, const double* __restrict__ partial, int64_t count, double max_norm, float* __restrict__ result) {
+  __shared__ float s_factor;
+  float norm, factor;
+  finish<KIND, kThreads>(partial, count, max_norm, norm, factor);
+  if (threadIdx.x == 0) {
+    s_factor = factor;
+    if (blockIdx.x == 0) {  // (of every launch of a long list: the same values)
+      result[0] = norm;
+      result[1] = factor;
+    }
+  }
+  __syncthreads();
+  scale_block<false>(l, gridDim.x - 1 - blockIdx.x, s_factor);
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host
@@ -257,17 +289,58 @@ bool list_ok(const void* const* in, const int64_t* numel, const int32_t* dtype, 
 }
 
 template <int KIND>
-int run_norm(const void* const* in, const int64_t* numel, const int32_t* dtype, int count, const Cut& c, double max_norm, float* result,
-             double* partial, hipStream_t stream) {
-  const int rc = for_each_run(in, nullptr, numel, dtype, nullptr, count, c, [&](const List& l, uint32_t blocks, int64_t before) {
+int run_partials(const void* const* in, const int64_t* numel, const int32_t* dtype, int count, const Cut& c, double* partial, hipStream_t stream) {
+  return for_each_run(in, nullptr, numel, dtype, nullptr, count, c, [&](const List& l, uint32_t blocks, int64_t before) {
     hipLaunchKernelGGL(norm_kernel<KIND>, dim3(blocks), dim3(kThreads), 0, stream, l, partial + before);
     NR_LAUNCH_CHECK();
     return 0;
   });
-  if (rc != 0) return rc;
-  hipLaunchKernelGGL(norm_finish_kernel<KIND>, dim3(1), dim3(kFinishThreads), 0, stream, partial, c.blocks, max_norm, result);
+}
+
+template <int KIND>
+int run_norm(const void* const* in, const int64_t* numel, const int32_t* dtype, int count, const Cut& c, double max_norm, float* result,
+             double* partial, hipStream_t stream) {
+  if (int rc = run_partials<KIND>(in, numel, dtype, count, c, partial, stream)) return rc;
+  if (c.blocks <= kFew)
+    hipLaunchKernelGGL((norm_finish_kernel<KIND, kThreads>), dim3(1), dim3(kThreads), 0, stream, partial, c.blocks, max_norm, result);
+  else
+    hipLaunchKernelGGL((norm_finish_kernel<KIND, kFinishThreads>), dim3(1), dim3(kFinishThreads), 0, stream, partial, c.blocks, max_norm, result);
   NR_LAUNCH_CHECK();
   return 0;
+}
+
+int run_scale(const void* const* grads, void* const* outs, const int64_t* numel, const int32_t* dtypes, const int32_t* out_dtypes, int count,
+              const Cut& c, const float* result, hipStream_t stream) {
+  int64_t bytes = 0;
+  for (int t = 0; t < count; ++t) bytes += numel[t] * (out_dtypes[t] == NR_DTYPE_F32 ? 4 : 2);
+  const bool past = bytes > kStreamBytes;
+  return for_each_run(grads, outs, numel, dtypes, out_dtypes, count, c, [&](const List& l, uint32_t blocks, int64_t) {
+    if (past) hipLaunchKernelGGL(scale_kernel<true>, dim3(blocks), dim3(kThreads), 0, stream, l, result);
+    else hipLaunchKernelGGL(scale_kernel<false>, dim3(blocks), dim3(kThreads), 0, stream, l, result);
+    NR_LAUNCH_CHECK();
+    return 0;
+  });
+}
+
+template <int KIND>
+int run_clip(const void* const* grads, void* const* outs, const int64_t* numel, const int32_t* dtypes, const int32_t* out_dtypes, int count,
+             const Cut& c, double max_norm, float* result, double* partial, hipStream_t stream) {
+  if (c.blocks == 0 || c.blocks > kFew) {
+    if (int rc = run_norm<KIND>(grads, numel, dtypes, count, c, max_norm, result, partial, stream)) return rc;
+    return run_scale(grads, outs, numel, dtypes, out_dtypes, count, c, result, stream);
+  }
+  if (int rc = run_partials<KIND>(grads, numel, dtypes, count, c, partial, stream)) return rc;
+  return for_each_run(grads, outs, numel, dtypes, out_dtypes, count, c, [&](const List& l, uint32_t blocks, int64_t) {
+    hipLaunchKernelGGL(finish_scale_kernel<KIND>, dim3(blocks), dim3(kThreads), 0, stream, l, partial, c.blocks, max_norm, result);
+    NR_LAUNCH_CHECK();
+    return 0;
+  });
+}
+
+bool norm_args_ok(const void* const* grads, const int64_t* numel, const int32_t* dtypes, int count, int norm_type, double max_norm,
+                  const float* result, const void* workspace, Cut* c) {
+  return cut_list(numel, count, c) && list_ok(grads, numel, dtypes, count) && norm_type >= 0 && norm_type <= 2 && max_norm >= 0.0 &&
+         result != nullptr && !(c->blocks > 0 && workspace == nullptr) && (reinterpret_cast<uintptr_t>(workspace) & 7) == 0;
 }
 
 }  // namespace
@@ -281,13 +354,9 @@ extern "C" int64_t nr_grad_norm_workspace_bytes(const int64_t* numel, int count)
 extern "C" int nr_grad_norm(const void* const* grads, const int64_t* numel, const int32_t* dtypes, int count, int norm_type, double max_norm,
                             float* result, void* workspace, nr_stream_t stream) {
   Cut c;
-  if (!cut_list(numel, count, &c) || !list_ok(grads, numel, dtypes, count) || norm_type < 0 || norm_type > 2 || !(max_norm >= 0.0) ||
-      result == nullptr || (c.blocks > 0 && workspace == nullptr) || (reinterpret_cast<uintptr_t>(workspace) & 7) != 0)
-    return NR_EINVAL;
-  double* partial = static_cast<double*>(workspace);
-  if (norm_type == kNormMax) return run_norm<kNormMax>(grads, numel, dtypes, count, c, max_norm, result, partial, nr_s(stream));
-  if (norm_type == kNormSum) return run_norm<kNormSum>(grads, numel, dtypes, count, c, max_norm, result, partial, nr_s(stream));
-  return run_norm<kNormTwo>(grads, numel, dtypes, count, c, max_norm, result, partial, nr_s(stream));
+  if (!norm_args_ok(grads, numel, dtypes, count, norm_type, max_norm, result, workspace, &c)) return NR_EINVAL;
+  auto run = norm_type == kNormMax ? run_norm<kNormMax> : norm_type == kNormSum ? run_norm<kNormSum> : run_norm<kNormTwo>;
+  return run(grads, numel, dtypes, count, c, max_norm, result, static_cast<double*>(workspace), nr_s(stream));
 }
 
 extern "C" int nr_grad_scale(const void* const* grads, void* const* outs, const int64_t* numel, const int32_t* dtypes, const int32_t* out_dtypes,
@@ -295,13 +364,14 @@ extern "C" int nr_grad_scale(const void* const* grads, void* const* outs, const 
   Cut c;
   if (!cut_list(numel, count, &c) || !list_ok(grads, numel, dtypes, count) || !list_ok(outs, numel, out_dtypes, count) || result == nullptr)
     return NR_EINVAL;
-  int64_t bytes = 0;
-  for (int t = 0; t < count; ++t) bytes += numel[t] * (out_dtypes[t] == NR_DTYPE_F32 ? 4 : 2);
-  const bool past = bytes > kStreamBytes;
-  return for_each_run(grads, outs, numel, dtypes, out_dtypes, count, c, [&](const List& l, uint32_t blocks, int64_t) {
-    if (past) hipLaunchKernelGGL(scale_kernel<true>, dim3(blocks), dim3(kThreads), 0, nr_s(stream), l, result);
-    else hipLaunchKernelGGL(scale_kernel<false>, dim3(blocks), dim3(kThreads), 0, nr_s(stream), l, result);
-    NR_LAUNCH_CHECK();
-    return 0;
-  });
+  return run_scale(grads, outs, numel, dtypes, out_dtypes, count, c, result, nr_s(stream));
+}
+
+extern "C" int nr_grad_clip(const void* const* grads, void* const* outs, const int64_t* numel, const int32_t* dtypes, const int32_t* out_dtypes,
+                            int count, int norm_type, double max_norm, float* result, void* workspace, nr_stream_t stream) {
+  Cut c;
+  if (!norm_args_ok(grads, numel, dtypes, count, norm_type, max_norm, result, workspace, &c) || !list_ok(outs, numel, out_dtypes, count))
+    return NR_EINVAL;
+  auto run = norm_type == kNormMax ? run_clip<kNormMax> : norm_type == kNormSum ? run_clip<kNormSum> : run_clip<kNormTwo>;
+  return run(grads, outs, numel, dtypes, out_dtypes, count, c, max_norm, result, static_cast<double*>(workspace), nr_s(stream));
 }

@@ -1349,8 +1349,8 @@ def _dense(t: Tensor) -> Tensor:
     return p if p.is_contiguous() else t.contiguous()
 
 
-def _norm_and_factor(lst: _GradList, max_norm: float, norm_type: float, device) -> Tensor:
-    """[norm, clip factor, ...] on the device."""
+def _norm_and_factor(lst: _GradList, max_norm: float, norm_type: float, device, out: Optional[_GradList] = None) -> Tensor:
+    """[norm, clip factor, ...] on the device; with `out` the gradients clipped into it."""
     kind = _NORM_TYPES.get(float(norm_type))
     if kind is None:
         raise RuntimeError(f"norm_type must be 1, 2 or infinity, not {norm_type}")
@@ -1362,8 +1362,11 @@ def _norm_and_factor(lst: _GradList, max_norm: float, norm_type: float, device) 
     if need < 0:
         raise RuntimeError("gradient list too long")
     workspace = torch.empty(2 + need // 4, device=device, dtype=torch.float32)  # [norm, factor | partial results]
-    at = workspace.data_ptr()
-    check(lib.nr_grad_norm(ptrs, numel, dtypes, lst.count, kind, max_norm, at, at + 8, _launch_stream(lst.device)), "nr_grad_norm")
+    at, stream = workspace.data_ptr(), _launch_stream(lst.device)
+    if out is None:
+        check(lib.nr_grad_norm(ptrs, numel, dtypes, lst.count, kind, max_norm, at, at + 8, stream), "nr_grad_norm")
+    else:
+        check(lib.nr_grad_clip(ptrs, out.arrays[0], numel, dtypes, out.arrays[2], lst.count, kind, max_norm, at, at + 8, stream), "nr_grad_clip")
     return workspace
 
 
@@ -1427,10 +1430,7 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> Tens
             dst = _GradList([o if o.is_contiguous() else torch.empty_like(o, memory_format=torch.contiguous_format) for o in targets], "out")
     if _lib.tensors().nr_same_address(dst.arrays[0], dst.count) != 0:
         raise RuntimeError("a tensor to be written is listed twice")
-    result = _norm_and_factor(src, float(max_norm), norm_type, device)
-    ptrs, numel, dtypes = src.arrays
-    check(_lib.lib().nr_grad_scale(ptrs, dst.arrays[0], numel, dtypes, dst.arrays[2], src.count, result.data_ptr(),
-                                   _launch_stream(src.device)), "nr_grad_scale")
+    result = _norm_and_factor(src, float(max_norm), norm_type, device, dst)
     if not dst.plain or dst.tensors is not targets:
         for target, written in zip(targets, dst.tensors):  # a target with holes gets its elements from a dense copy
             if written.data_ptr() != target.data_ptr():

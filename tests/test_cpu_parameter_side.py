@@ -53,6 +53,11 @@ def test_norm_entry_points_refuse_bad_arguments():
         assert norm(**kw) == E, kw
     for kw in (dict(o=None), dict(od=None), dict(result=None), dict(o=array("q", [0, BIG])), dict(o=array("q", [BIG, BIG + 1]))):
         assert scale(**kw) == E, kw
+    def clip(o=ptrs, od=dtypes, kind=2, max_norm=1.0, result=BIG, workspace=BIG):
+        return lib.nr_grad_clip(at(ptrs), o and at(o), at(numel), at(dtypes), od and at(od), 2, kind, max_norm, result, workspace, None)
+
+    for kw in (dict(o=None), dict(od=None), dict(kind=5), dict(max_norm=-2.0), dict(result=None), dict(workspace=None), dict(o=array("q", [BIG, BIG + 1]))):
+        assert clip(**kw) == E, kw
     assert lib.nr_grad_norm_workspace_bytes(at(numel), -1) == E and lib.nr_grad_norm_workspace_bytes(at(array("q", [-5])), 1) == E
     assert lib.nr_grad_norm_workspace_bytes(None, 0) == 0 and lib.nr_grad_norm_workspace_bytes(at(numel), 2) == 16
 

@@ -58,7 +58,7 @@ def test_norm_and_clip(sizes, dtypes):
             out = [torch.full_like(g, 9.0) for g in grads]
             check_clip(out, grads, ratio * n64, p, ops.clip_grads(grads, ratio * n64, p, out=out))
             mine = [g.clone() for g in grads]
-            norm = ops.clip_grads(mine, ratio * n64, p)
+            assert torch.equal(norm, ops.clip_grads(mine, ratio * n64, p))  # (with the factor formed in the scaling launch as well)
             assert all(torch.equal(a, b) for a, b in zip(mine, out)) and (ratio < 1 or all(torch.equal(a, b) for a, b in zip(mine, grads)))
 
 
@@ -167,3 +167,21 @@ def test_refusals():
         with pytest.raises(RuntimeError, match=what):
             call()
     assert bool((g == 1).all())
+
+
+def test_norm_and_scale_as_separate_calls():
+    """The C entry points one after the other (a caller that keeps the factor): the same bits as in one call."""
+    from neuradar_amd import _lib
+
+    for sizes in ((5000, 7, 123457), (40000000, 3)):  # (few partial results, and thousands of them)
+        grads = ragged(sizes, (F32, BF16))
+        lst = ops._GradList(grads, "gradients")
+        outs = [torch.empty_like(g) for g in grads]
+        dst = ops._GradList(outs, "out")
+        result = ops._norm_and_factor(lst, 0.5, 2.0, grads[0].device)
+        lib = _lib.lib()
+        assert lib.nr_grad_scale(lst.arrays[0], dst.arrays[0], lst.arrays[1], lst.arrays[2], dst.arrays[2], 2 if len(sizes) == 2 else 3, result.data_ptr(),
+                                 torch.cuda.current_stream().cuda_stream) == 0
+        other = [torch.empty_like(g) for g in grads]
+        assert torch.equal(ops.clip_grads(grads, 0.5, out=other), result[0])
+        assert all(torch.equal(a, b) for a, b in zip(outs, other))
