@@ -275,3 +275,11 @@ def test_two_streams_at_once_and_no_second_derivative():
     (first,) = torch.autograd.grad(ops.embedding(table, torch.tensor([1, 2], device=DEV)).square().sum(), table, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable|does not require grad|differentiable"):
         first.sum().backward()
+
+
+def test_rows_beyond_the_caches():
+    """More than 256 MB of rows leave past the caches: whole and odd widths, the last vector of a row among them."""
+    for dim in (257, 512):
+        table = (torch.randn(5000, dim, generator=torch.Generator().manual_seed(dim)) * 0.5).to(BF16).to(DEV)
+        idx = torch.randint(0, 5000, (300_000_000 // (2 * dim),), device=DEV)
+        assert torch.equal(ops.embedding(table, idx, 3.0), (table.float() * 3.0).to(BF16)[idx])

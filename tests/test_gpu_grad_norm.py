@@ -173,7 +173,7 @@ def test_norm_and_scale_as_separate_calls():
     """The C entry points one after the other (a caller that keeps the factor): the same bits as in one call."""
     from neuradar_amd import _lib
 
-    for sizes in ((5000, 7, 123457), (40000000, 3)):  # (few partial results, and thousands of them)
+    for sizes in ((5000, 7, 123457), (40000000, 3), (75000001, 5)):  # (few partial results, thousands, results beyond the caches)
         grads = ragged(sizes, (F32, BF16))
         lst = ops._GradList(grads, "gradients")
         outs = [torch.empty_like(g) for g in grads]
@@ -184,4 +184,4 @@ def test_norm_and_scale_as_separate_calls():
                                  torch.cuda.current_stream().cuda_stream) == 0
         other = [torch.empty_like(g) for g in grads]
         assert torch.equal(ops.clip_grads(grads, 0.5, out=other), result[0])
-        assert all(torch.equal(a, b) for a, b in zip(outs, other))
+        assert all(torch.equal(a, b) and torch.equal(a, (g.float() * result[1]).to(g.dtype)) for a, b, g in zip(outs, other, grads))
