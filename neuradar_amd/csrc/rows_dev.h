@@ -39,25 +39,105 @@ __device__ __forceinline__ void nr_store_pack_stream(T* __restrict__ p, const fl
 // whoever reads them next, and writing them past it leaves it to the inputs.  Measured: 537 MB of rows from a table of 268 MB
 // 171 -> 114 us; a norm (613 MB) after a scaling that wrote as much 124 -> 94 us; 134 MB the same either way.
 constexpr int64_t kStreamBytes = (int64_t)256 << 20;
-// the first m of N elements (the end of a row or of a tensor)
+
+// The first m of N elements (the end of a row or of a tensor): 8, 4 and 2 bytes, up to three accesses and not m.  The vector
+// is held as two integers that are shifted, never as an array that is indexed, so that it stays in registers.  Measured against one
+// element at a time: a gradient of 4 594 rows of 223 bf16 values 40 -> 25 us, a lookup of 200 000 rows of 13 fp16 values 8.4 -> 6.0.
+template <typename W, typename T>
+struct NrPiece {
+  typedef W __attribute__((may_alias, aligned(alignof(T)))) type;
+};
 template <typename T, int N>
 __device__ __forceinline__ void nr_load_some(const T* __restrict__ p, int m, float (&x)[N]) {
   if (m >= N) {
     nr_load_pack<T, N>(p, x);
-  } else {
-#pragma unroll
-    for (int k = 0; k < N; ++k) x[k] = k < m ? (float)p[k] : 0.0f;
+    return;
   }
+  if constexpr (N * sizeof(T) > 16) {
+    float half[N / 2], rest[N / 2];
+    nr_load_some<T, N / 2>(p, m, half);
+    nr_load_some<T, N / 2>(p + N / 2, m > N / 2 ? m - N / 2 : 0, rest);
+#pragma unroll
+    for (int k = 0; k < N / 2; ++k) {
+      x[k] = half[k];
+      x[N / 2 + k] = rest[k];
+    }
+    return;
+  }
+  const int bytes = m * (int)sizeof(T);
+  const char* at = reinterpret_cast<const char*>(p);
+  uint64_t low = 0, eight = 0;
+  if (bytes & 8) {
+    eight = *reinterpret_cast<const typename NrPiece<uint64_t, T>::type*>(at);
+    at += 8;
+  }
+  if (bytes & 4) {
+    low = *reinterpret_cast<const typename NrPiece<uint32_t, T>::type*>(at);
+    at += 4;
+  }
+  if (sizeof(T) == 2 && (bytes & 2)) {
+    const uint64_t two = *reinterpret_cast<const typename NrPiece<uint16_t, T>::type*>(at);
+    low |= (bytes & 4) ? two << 32 : two;
+  }
+  typedef uint64_t two64 __attribute__((ext_vector_type(2)));
+  const two64 all = {(bytes & 8) ? eight : low, (bytes & 8) ? low : 0};
+  typedef T whole __attribute__((ext_vector_type(16 / sizeof(T))));
+  const whole v = __builtin_bit_cast(whole, all);
+#pragma unroll
+  for (int k = 0; k < N && k < (int)(16 / sizeof(T)); ++k) x[k] = (float)v[k];
 }
 template <typename T, int N>
 __device__ __forceinline__ void nr_store_some(T* __restrict__ p, int m, const float (&x)[N]) {
   if (m >= N) {
     nr_store_pack<T, N>(p, x);
-  } else {
-#pragma unroll
-    for (int k = 0; k < N; ++k)
-      if (k < m) p[k] = (T)x[k];
+    return;
   }
+  if constexpr (N * sizeof(T) > 16) {
+    float half[N / 2], rest[N / 2];
+#pragma unroll
+    for (int k = 0; k < N / 2; ++k) {
+      half[k] = x[k];
+      rest[k] = x[N / 2 + k];
+    }
+    nr_store_some<T, N / 2>(p, m, half);
+    nr_store_some<T, N / 2>(p + N / 2, m > N / 2 ? m - N / 2 : 0, rest);
+    return;
+  }
+  typedef uint64_t two64 __attribute__((ext_vector_type(2)));
+  typedef T whole __attribute__((ext_vector_type(16 / sizeof(T))));
+  whole v = {};
+#pragma unroll
+  for (int k = 0; k < N && k < (int)(16 / sizeof(T)); ++k) v[k] = (T)x[k];
+  const two64 all = __builtin_bit_cast(two64, v);
+  const int bytes = m * (int)sizeof(T);
+  char* at = reinterpret_cast<char*>(p);
+  uint64_t low = all[0];
+  if (bytes & 8) {
+    *reinterpret_cast<typename NrPiece<uint64_t, T>::type*>(at) = low;
+    at += 8;
+    low = all[1];
+  }
+  if (bytes & 4) {
+    *reinterpret_cast<typename NrPiece<uint32_t, T>::type*>(at) = (uint32_t)low;
+    at += 4;
+    low >>= 32;
+  }
+  if (sizeof(T) == 2 && (bytes & 2)) *reinterpret_cast<typename NrPiece<uint16_t, T>::type*>(at) = (uint16_t)low;
+}
+
+// N floats in LDS, 16-byte aligned
+template <int N>
+__device__ __forceinline__ void nr_lds_get(const float* p, float (&x)[N]) {
+#pragma unroll
+  for (int q = 0; q < N / 4; ++q) {
+    const float4 v = reinterpret_cast<const float4*>(p)[q];
+    x[q * 4] = v.x; x[q * 4 + 1] = v.y; x[q * 4 + 2] = v.z; x[q * 4 + 3] = v.w;
+  }
+}
+template <int N>
+__device__ __forceinline__ void nr_lds_put(float* p, const float (&x)[N]) {
+#pragma unroll
+  for (int q = 0; q < N / 4; ++q) reinterpret_cast<float4*>(p)[q] = make_float4(x[q * 4], x[q * 4 + 1], x[q * 4 + 2], x[q * 4 + 3]);
 }
 
 }  // namespace
