@@ -35,8 +35,10 @@ constexpr int64_t kZeroBlocks = 2048;                 // blocks of a launch that
 // ---------------------------------------------------------------------------------------------------------------- rows
 constexpr int kRowUnroll = 4;
 
-// Flat over the 16-byte vectors of the output, four per thread: every lane has work whatever the width is.  A row's last vector
-// may be short (dim not a multiple of the vector): element by element.
+// Flat over the 16-byte vectors of the output, four per thread: every lane has work whatever the width is.  Where dim is not a
+// multiple of the vector a row's last one starts earlier and lies over the one before (both write the same values there), so that
+// every access is a whole vector; only rows shorter than a vector are taken in pieces.  (200 000 rows of 13 fp16 values: 6.0 -> 4.6 us,
+// 50 021 rows of 33 4.3 -> 3.7, against a last vector in pieces.)
 template <typename T, typename I, bool STREAM>
 __global__ void __launch_bounds__(kThreads)
 rows_kernel(const T* __restrict__ table, int64_t rows, int dim, int64_t row_stride, const I* __restrict__ idx, int64_t n, float scale,
@@ -52,14 +54,16 @@ rows_kernel(const T* __restrict__ table, int64_t rows, int dim, int64_t row_stri
     const uint32_t l = rem0 + (uint32_t)(u * kThreads) + threadIdx.x;
     const uint32_t q = magic == 0u ? l : __umulhi(l, magic);
     r[u] = row0 + q;
-    col[u] = (int)(l - q * nv) * N;
+    col[u] = max(min((int)(l - q * nv) * N, dim - N), 0);
     v[u] = r[u] < n ? (int64_t)idx[r[u]] : -1;
   }
   float x[kRowUnroll][N];
 #pragma unroll
   for (int u = 0; u < kRowUnroll; ++u) {
     if (v[u] >= 0 && v[u] < rows) {
-      nr_load_some<T, N>(table + v[u] * row_stride + col[u], dim - col[u], x[u]);
+      const T* t = table + v[u] * row_stride + col[u];
+      if (dim >= N) nr_load_pack<T, N>(t, x[u]);
+      else nr_load_some<T, N>(t, dim, x[u]);
     } else {
 #pragma unroll
       for (int k = 0; k < N; ++k) x[u][k] = __builtin_nanf("");
@@ -71,8 +75,9 @@ rows_kernel(const T* __restrict__ table, int64_t rows, int dim, int64_t row_stri
 #pragma unroll
     for (int k = 0; k < N; ++k) x[u][k] *= scale;
     T* o = out + r[u] * out_stride + col[u];
-    if (STREAM && dim - col[u] >= N) nr_store_pack_stream<T, N>(o, x[u]);
-    else nr_store_some<T, N>(o, dim - col[u], x[u]);
+    if (dim < N) nr_store_some<T, N>(o, dim, x[u]);
+    else if (STREAM) nr_store_pack_stream<T, N>(o, x[u]);
+    else nr_store_pack<T, N>(o, x[u]);
   }
 }
 
@@ -312,11 +317,15 @@ constexpr int kFlight = 8;         // rows of g requested before the first of th
 // One group's stretch [q0, q1) of sorted tokens, on its columns: sums that start and end inside are written; a first sum that
 // started before the stretch is left in `head`, a last one that goes on behind it in `tail`.  key_at(q): the key of token q, also
 // of the one before the stretch and the one behind it; pos_at(q): its row of g.  Returns kHead | kSpan | kTail.  (Keys and
-// positions of a batch are read before anything is written: the compiler cannot know that a result is not one of them.)
+// positions of a batch are read before anything is written: the compiler cannot know that a result is not one of them.)  A
+// row's last vector is read whole too, from as many columns earlier as it lacks, and its sum is moved into place at its end
+// (131 072 x 513 bf16: 141 -> 119 us against pieces, whose branches keep the rows of a flight from being requested together).
 template <typename T, int N, typename Key, typename Pos>
 __device__ __forceinline__ uint32_t walk_stretch(const SumArgs& a, const T* __restrict__ grad, int q0, int q1, int col, uint32_t row0, Key key_at,
                                                  Pos pos_at, float* head, float* tail) {
   uint32_t flag = 0u;
+  const int back = a.dim >= N ? max(col + N - a.dim, 0) : 0;
+  const T* from = grad + (col - back);
   float acc[N];
 #pragma unroll
   for (int k = 0; k < N; ++k) acc[k] = 0.0f;
@@ -334,8 +343,12 @@ __device__ __forceinline__ uint32_t walk_stretch(const SumArgs& a, const T* __re
       key[u + 1] = in ? key_at(q + u + 1) : 0u;
     }
 #pragma unroll
-    for (int u = 0; u < kFlight; ++u)
-      if (q + u < q1) nr_load_some<T, N>(grad + (int64_t)pos[u] * a.grad_stride + col, a.dim - col, x[u]);
+    for (int u = 0; u < kFlight; ++u) {
+      if (q + u >= q1) continue;
+      const T* row = from + (int64_t)pos[u] * a.grad_stride;
+      if (a.dim >= N) nr_load_pack<T, N>(row, x[u]);
+      else nr_load_some<T, N>(row, a.dim, x[u]);
+    }
 #pragma unroll
     for (int u = 0; u < kFlight; ++u) {
       if (q + u >= q1) break;
@@ -343,6 +356,12 @@ __device__ __forceinline__ uint32_t walk_stretch(const SumArgs& a, const T* __re
 #pragma unroll
       for (int k = 0; k < N; ++k) acc[k] += x[u][k];
       if (goes_on && q + u + 1 < q1) continue;
+#pragma unroll
+      for (int step = 1; step < N; step *= 2) {
+        if ((back & step) == 0) continue;
+#pragma unroll
+        for (int k = 0; k + step < N; ++k) acc[k] = acc[k + step];
+      }
       float* part = nullptr;
       if (!open_here) {
         part = head;
