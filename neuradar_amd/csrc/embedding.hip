@@ -18,8 +18,8 @@
 //     group, one that leaves the block is left in the workspace and added up in block order by a last launch.
 // Bound by memory where rows are long (read g once, write the table once), by the chain of launches and of dependent steps inside
 // a block where they are few.  Measured, kernels alone: rows 262 144 x 1 024 bf16 114 us (0.69 GB of traffic: 6.0 TB/s; 153 us on
-// a cold table); gradient 16 384 x 16 on 60 rows 12 us, 113 840 x 32 on 1 999 rows 21 + 4, 8 192 x 8 on 2^22 rows 27 (134 MB of
-// zeros alone: 18), 100 003 x 257 on 7 rows 34 + 5 (103 MB: 20), 131 072 x 512 bf16 on 131 072 rows 108 (sort 45, which also
+// a cold table); gradient 16 384 x 16 on 60 rows 11 us, 113 840 x 32 on 1 999 rows 18 + 4, 8 192 x 8 on 2^22 rows 25 (134 MB of
+// zeros alone: 18), 100 003 x 257 on 7 rows 32 + 4 (103 MB: 20), 131 072 x 512 bf16 on 131 072 rows 108 (sort 45, which also
 // writes the zeros; sums 53 at 3.2 TB/s; join 9).
 #include "rows_dev.h"
 

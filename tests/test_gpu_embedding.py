@@ -283,3 +283,27 @@ def test_rows_beyond_the_caches():
         table = (torch.randn(5000, dim, generator=torch.Generator().manual_seed(dim)) * 0.5).to(BF16).to(DEV)
         idx = torch.randint(0, 5000, (300_000_000 // (2 * dim),), device=DEV)
         assert torch.equal(ops.embedding(table, idx, 3.0), (table.float() * 3.0).to(BF16)[idx])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=str)
+def test_row_ends_of_every_width(dtype):
+    """A row's last vector is read and written over the one before: widths around the vectors' own, rows that start one element off,
+    NaN before and behind every row, all three ways of the gradient, added to what is there too.  Small whole numbers: exact in
+    every type (a row's sum: at most 20 * 2 + 3 < 2^8), so nothing may differ at all."""
+    gen = torch.Generator().manual_seed(41)
+    for dim in [*range(1, 20), 31, 33, 63, 65]:
+        for n, rows in ((5, 3), (500, 90), (17000, 6000), (17000, 900000)):
+            idx = torch.randint(0, rows, (n,), generator=gen)
+            idx = idx[torch.bincount(idx, minlength=rows)[idx] <= 20]
+            n = len(idx)
+            wide = torch.full((n + 1, dim + 3), float("nan"), dtype=dtype)
+            wide[:n, 1:dim + 1] = torch.randint(-2, 3, (n, dim), generator=gen).to(dtype)
+            grad = wide.to(DEV)[:n, 1:dim + 1]
+            want = torch.zeros(rows, dim).index_add_(0, idx, wide[:n, 1:dim + 1].float())
+            got = ops.embedding_grad(grad, idx.to(DEV), rows)
+            assert torch.equal(got.float().cpu(), want), (dim, n, rows)
+            out = torch.full((rows, dim), 3.0, dtype=dtype, device=DEV)
+            ops.embedding_grad(grad, idx.to(DEV), rows, out=out, accumulate=True)
+            assert torch.equal(out.float().cpu(), want + 3.0), (dim, n, rows)
+            back = torch.randint(0, n, (n + 7,), generator=gen)
+            assert torch.equal(ops.embedding(grad, back.to(DEV)).cpu(), wide[:n, 1:dim + 1][back]), (dim, n)
