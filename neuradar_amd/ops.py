@@ -10,6 +10,7 @@ from typing import List, Optional, Sequence, Tuple
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -728,6 +729,12 @@ def _row_index(idx: Tensor, device: int) -> Tensor:
     return idx.contiguous()
 
 
+def _differentiated(t: Tensor) -> bool:
+    """Whether autograd follows `t`, backwards or forwards.  (A dual tensor of forward mode does not require grad; the level is asked
+    first, 0.1 us, because outside of one no tensor has a tangent.)"""
+    return (t.requires_grad and torch.is_grad_enabled()) or (forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None)
+
+
 def _padding_row(padding_idx: Optional[int], rows: int) -> int:
     """nn.Embedding's convention: negative counts from the end; -1 (none) for the ABI."""
     if padding_idx is None:
@@ -823,12 +830,12 @@ def embedding(table: Tensor, idx: Tensor, scale: float = 1.0, padding_idx: Optio
     """scale * table[idx]: rows of an embedding table [rows, dim] (fp32 / bf16 / fp16; rows may be apart, columns neighbours) for
     indices of any shape (int64 / int32) -> [*idx.shape, dim] in the table's type, one rounding.  An index outside [0, rows) gives
     a row of NaN and no gradient (nothing is read on the host, so nothing can be raised).
-    Differentiable in the table: embedding_grad, inside `direct_param_grads` straight into table.grad.  padding_idx as in
-    nn.Embedding: that row is looked up like any other and gets no gradient."""
+    Differentiable in the table, backwards and once: embedding_grad, inside `direct_param_grads` straight into table.grad.
+    padding_idx as in nn.Embedding: that row is looked up like any other and gets no gradient."""
     _float_rows(table, "table")
     idx = _row_index(idx, table.get_device())
     _padding_row(padding_idx, table.shape[0])
-    if table.requires_grad and torch.is_grad_enabled():
+    if _differentiated(table):  # (forward mode raises in there: there is no formula for it)
         return _Embedding.apply(table, idx, float(scale), padding_idx)
     return _embedding_rows(table, idx, float(scale))
 

@@ -1,0 +1,31 @@
+"""CPU (no GPU): no derivative through the embedding, norm and clipping entry points is lost without an error."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from neuradar_amd import ops
+
+
+@pytest.fixture
+def rows_on_the_cpu(monkeypatch):
+    """ops.embedding with its launch replaced by torch on detached values (what the kernel does: it sees addresses)."""
+    monkeypatch.setattr(ops, "_float_rows", lambda t, what: t)
+    monkeypatch.setattr(ops, "_row_index", lambda idx, device: idx)
+    monkeypatch.setattr(ops, "_embedding_rows", lambda table, idx, scale: forward_ad.unpack_dual(table).primal.detach()[idx] * scale)
+
+
+def test_a_tangent_is_not_dropped(rows_on_the_cpu):
+    table, idx = torch.randn(4, 3), torch.tensor([1, 1, 3])
+    for requires_grad in (False, True):
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(table.clone().requires_grad_(requires_grad), torch.ones(4, 3))
+            with pytest.raises(NotImplementedError):
+                ops.embedding(dual, idx, 2.0)
+            with torch.no_grad(), pytest.raises(NotImplementedError):  # (forward mode goes on under no_grad)
+                ops.embedding(dual, idx, 2.0)
+            assert torch.equal(ops.embedding(table, idx, 2.0), table[idx] * 2.0)  # a tensor without a tangent
+    assert ops.embedding(table, idx).grad_fn is None
+    leaf = table.clone().requires_grad_()
+    assert ops.embedding(leaf, idx).grad_fn is not None
+    with torch.no_grad():
+        assert ops.embedding(leaf, idx).grad_fn is None
