@@ -266,13 +266,15 @@ _tensors = None
 
 
 def tensors() -> ctypes.PyDLL:
-    """libneuradar_tensors.so: nr_tensor_list and nr_same_address (csrc/tensor_list.cpp), called with the interpreter lock held."""
+    """libneuradar_tensors.so: nr_tensor_list, nr_mark_written and nr_same_address (csrc/tensor_list.cpp), called with the interpreter
+    lock held."""
     global _tensors
     if _tensors is None:
         if not os.path.exists(TENSORS_PATH):
             raise RuntimeError(f"{TENSORS_PATH} is missing. Build it with `make -C neuradar_amd/csrc`.")
         handle = ctypes.PyDLL(TENSORS_PATH)
         handle.nr_tensor_list.argtypes = [ctypes.py_object, P, P, P]
+        handle.nr_mark_written.argtypes = [ctypes.py_object]
         handle.nr_same_address.argtypes = [P, L]
         _tensors = handle
     return _tensors

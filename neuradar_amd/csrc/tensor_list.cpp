@@ -41,6 +41,21 @@ extern "C" int nr_tensor_list(PyObject* list, int64_t* ptr, int64_t* numel, int3
   }
 }
 
+// The list's tensors have been written through their addresses: autograd's version counters go up, as after any write in place, so
+// that a backward pass that saved one of them raises.  (A tensor of inference mode has no counter.)
+extern "C" int nr_mark_written(PyObject* list) {
+  try {
+    const Py_ssize_t n = PyList_GET_SIZE(list);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      const at::Tensor& t = THPVariable_Unpack(PyList_GET_ITEM(list, i));
+      if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    }
+    return 0;
+  } catch (...) {
+    return kFailed;
+  }
+}
+
 // 1 if two of the non-empty tensors start at the same address.
 extern "C" int nr_same_address(const int64_t* ptr, int64_t n) {
   try {

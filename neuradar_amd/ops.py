@@ -781,6 +781,7 @@ def embedding_grad(grad: Tensor, idx: Tensor, num_rows: int, scale: float = 1.0,
     grad = _float_rows(grad if grad.dim() == 2 else grad.reshape(n, dim), "grad")
     idx = _row_index(idx, device)
     padding = _padding_row(padding_idx, num_rows)
+    given = out is not None
     if out is None:
         if accumulate:
             raise RuntimeError("accumulate=True adds to `out`: give it")
@@ -802,6 +803,8 @@ def embedding_grad(grad: Tensor, idx: Tensor, num_rows: int, scale: float = 1.0,
     check(lib.nr_embedding_bwd(grad.data_ptr(), code, stride, idx.data_ptr(), idx.element_size(), n, num_rows, dim, float(scale), padding,
                                out.data_ptr(), _DTYPE_CODES[out.dtype], accumulate, None if workspace is None else workspace.data_ptr(),
                                _launch_stream(device)), "nr_embedding_bwd")
+    if given:
+        torch.autograd.graph.increment_version(out)  # (written through its address)
     return out
 
 
@@ -1412,7 +1415,8 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> Tens
     """Scale gradients by min(1, max_norm / (norm + 1e-6)), norm = grad_norm(grads, norm_type), which is returned.  In place, or
     into the tensors of `out` (as many elements each, any of the three types: places in a 16-bit bucket, say), one rounding.
     Nothing is read on the host; a norm of NaN makes every gradient NaN, as in torch.  Tensors that are written must not share
-    memory (two that start at one address are refused)."""
+    memory (two that start at one address are refused).  A graph that saved a tensor which is written here raises when it
+    is differentiated."""
     grads = _as_list(grads)
     targets = grads if out is None else _as_list(out)
     if len(targets) != len(grads):
@@ -1438,6 +1442,7 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> Tens
     if _lib.tensors().nr_same_address(dst.arrays[0], dst.count) != 0:
         raise RuntimeError("a tensor to be written is listed twice")
     result = _norm_and_factor(src, float(max_norm), norm_type, device, dst)
+    _lib.tensors().nr_mark_written(targets)
     if not dst.plain or dst.tensors is not targets:
         for target, written in zip(targets, dst.tensors):  # a target with holes gets its elements from a dense copy
             if written.data_ptr() != target.data_ptr():

@@ -3,7 +3,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from neuradar_amd import ops
+from neuradar_amd import _lib, ops
 
 
 @pytest.fixture
@@ -29,3 +29,18 @@ def test_a_tangent_is_not_dropped(rows_on_the_cpu):
     assert ops.embedding(leaf, idx).grad_fn is not None
     with torch.no_grad():
         assert ops.embedding(leaf, idx).grad_fn is None
+
+
+def test_written_tensors_are_marked():
+    x, y = torch.randn(3), torch.randn(2)
+    before = x._version, y._version
+    with torch.inference_mode():
+        inferred = torch.randn(2)  # (has no counter)
+    assert _lib.tensors().nr_mark_written([x, inferred, y]) == 0
+    assert x._version > before[0] and y._version > before[1]
+    leaf = torch.randn(3, requires_grad=True)
+    (g,) = torch.autograd.grad((leaf ** 3).sum(), leaf, create_graph=True)
+    z = (g * g).sum()  # saves g
+    _lib.tensors().nr_mark_written([g])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
