@@ -1,6 +1,7 @@
 // Addresses, sizes and types of a Python list of tensors (host code): what nr_grad_norm / nr_grad_scale take, read in one call.
 // Asking every tensor for four things from Python costs a microsecond each, which for a few hundred gradients is more than the
 // kernels take.  Called with the interpreter lock held (ctypes.PyDLL); nothing is thrown across the boundary.
+#include <c10/core/GradMode.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
@@ -8,16 +9,18 @@
 #include <vector>
 
 namespace {
-enum { kNotTensors = -1, kType = -2, kDevice = -3, kLayout = -4, kFailed = -5 };
+enum { kNotTensors = -1, kType = -2, kDevice = -3, kLayout = -4, kFailed = -5, kTracked = -6 };
 }
 
 // ptr, numel [len(list)], dtype [len(list)] (NR_DTYPE_*) <- the list's.  Returns the one device that they are on; or kNotTensors;
-// kType: one is not fp32 / bf16 / fp16; kDevice: not all on one GPU; kLayout: one is not contiguous (its address is not taken).
+// kType: one is not fp32 / bf16 / fp16; kTracked: autograd follows one, backwards or forwards; kDevice: not all on one GPU; kLayout:
+// one is not contiguous (its address is not taken).
 extern "C" int nr_tensor_list(PyObject* list, int64_t* ptr, int64_t* numel, int32_t* dtype) {
   try {
     if (!PyList_Check(list)) return kNotTensors;
     int device = -1;
     bool dense = true;
+    const bool grad_mode = c10::GradMode::is_enabled();
     const Py_ssize_t n = PyList_GET_SIZE(list);
     for (Py_ssize_t i = 0; i < n; ++i) {
       PyObject* o = PyList_GET_ITEM(list, i);
@@ -29,6 +32,7 @@ extern "C" int nr_tensor_list(PyObject* list, int64_t* ptr, int64_t* numel, int3
         case at::kHalf: dtype[i] = 2; break;
         default: return kType;
       }
+      if ((grad_mode && t.requires_grad()) || t._fw_grad(0).defined()) return kTracked;
       if (!t.is_cuda() || (device >= 0 && t.get_device() != device)) return kDevice;
       device = (int)t.get_device();
       numel[i] = t.numel();

@@ -770,7 +770,10 @@ def embedding_grad(grad: Tensor, idx: Tensor, num_rows: int, scale: float = 1.0,
     indices -- no atomics, the same bits on every call.  grad [*idx.shape, dim] (rows may be apart), fp32 / bf16 / fp16; sums in
     fp32, rounded once to the result's type (`dtype`; grad's own by default).
     out: contiguous [num_rows, dim] that takes the result; accumulate: added to what `out` holds (rows that no index names are not
-    touched).  Indices equal to padding_idx or outside [0, num_rows) contribute nothing."""
+    touched).  Indices equal to padding_idx or outside [0, num_rows) contribute nothing.  Not differentiable: grad or out that autograd
+    follows are refused (under torch.no_grad() they are not)."""
+    if _differentiated(grad) or (out is not None and _differentiated(out)):
+        raise RuntimeError("embedding_grad has no derivative: call it under torch.no_grad() or on detached tensors")
     device = grad.get_device()
     if device >= 0 and device != _current_device():
         with torch.cuda.device(device):
@@ -1344,7 +1347,9 @@ class _GradList:
             self.device = _lib.tensors().nr_tensor_list(self.tensors, *self.arrays)
         if self.device < 0 and n > 0:
             raise RuntimeError({-1: f"{what} must be tensors", -2: f"{what} must be float32, bfloat16 or float16",
-                                -3: f"{what} must be GPU tensors on one device: neuradar_amd has no CPU path (the oracle is test-only)"}
+                                -3: f"{what} must be GPU tensors on one device: neuradar_amd has no CPU path (the oracle is test-only)",
+                                -6: f"{what} that autograd follows: the norm and the clipping have no derivative, call them under "
+                                    "torch.no_grad() or on detached tensors"}
                                .get(self.device, f"{what} cannot be read"))
 
 
@@ -1386,7 +1391,8 @@ def _as_list(tensors) -> List[Tensor]:
 
 def grad_norm(grads, norm_type: float = 2.0) -> Tensor:
     """Global norm (norm_type 2, 1 or infinity) over all elements of a tensor or of a sequence of tensors (fp32 / bf16 / fp16, mixed)
-    -> fp32 scalar tensor.  Two launches for up to 96 tensors; nothing is read on the host; sums in fp64 in a fixed order."""
+    -> fp32 scalar tensor.  Two launches for up to 96 tensors; nothing is read on the host; sums in fp64 in a fixed order.  Not
+    differentiable: tensors that autograd follows are refused (under torch.no_grad() they are not)."""
     grads = _as_list(grads)
     if not grads:
         return torch.zeros((), device="cuda", dtype=torch.float32)
@@ -1399,7 +1405,7 @@ def grad_norm(grads, norm_type: float = 2.0) -> Tensor:
 
 def clip_factor(grads, max_norm: float, norm_type: float = 2.0) -> Tuple[Tensor, Tensor]:
     """(norm, min(1, max_norm / (norm + 1e-6))) as fp32 tensors of one element each, the gradients untouched: for an optimizer that
-    multiplies them itself (adam_step's `clip`), which saves the pass that clip_grads makes over them."""
+    multiplies them itself (adam_step's `clip`), which saves the pass that clip_grads makes over them.  Not differentiable, as grad_norm."""
     grads = _as_list(grads)
     if not grads:
         raise RuntimeError("clip_factor: no gradients")
@@ -1415,8 +1421,8 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> Tens
     """Scale gradients by min(1, max_norm / (norm + 1e-6)), norm = grad_norm(grads, norm_type), which is returned.  In place, or
     into the tensors of `out` (as many elements each, any of the three types: places in a 16-bit bucket, say), one rounding.
     Nothing is read on the host; a norm of NaN makes every gradient NaN, as in torch.  Tensors that are written must not share
-    memory (two that start at one address are refused).  A graph that saved a tensor which is written here raises when it
-    is differentiated."""
+    memory (two that start at one address are refused).  Not differentiable: tensors that autograd follows are refused (under
+    torch.no_grad() they are not); a graph that saved a tensor which is written here raises when it is differentiated."""
     grads = _as_list(grads)
     targets = grads if out is None else _as_list(out)
     if len(targets) != len(grads):

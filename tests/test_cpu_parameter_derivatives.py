@@ -31,6 +31,21 @@ def test_a_tangent_is_not_dropped(rows_on_the_cpu):
         assert ops.embedding(leaf, idx).grad_fn is None
 
 
+def test_calls_without_a_derivative_refuse_tensors_that_autograd_follows():
+    leaf, plain, idx = torch.randn(3, 2, requires_grad=True), torch.randn(3, 2), torch.tensor([0, 1, 1])
+    calls = [lambda x: ops.grad_norm([x, plain]), lambda x: ops.clip_factor([x], 1.0), lambda x: ops.clip_grads([x], 1.0),
+             lambda x: ops.clip_grads([x], 1.0, out=[plain]), lambda x: ops.embedding_grad(x, idx, 4),
+             lambda x: ops.embedding_grad(plain, idx, 3, out=x)]
+    for call in calls:
+        for x in (leaf, leaf * 2.0):
+            with pytest.raises(RuntimeError, match="derivative"):
+                call(x)
+        with forward_ad.dual_level(), pytest.raises(RuntimeError, match="derivative"):
+            call(forward_ad.make_dual(plain.clone(), torch.ones(3, 2)))
+        with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU path"):  # (not followed: on to the next check)
+            call(leaf)
+
+
 def test_written_tensors_are_marked():
     x, y = torch.randn(3), torch.randn(2)
     before = x._version, y._version

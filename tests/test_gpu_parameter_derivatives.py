@@ -1,6 +1,7 @@
-"""GPU: a tensor written by clipping or by a gradient into `out` is a write in place to autograd."""
+"""GPU: a tensor written by clipping or by a gradient into `out` is a write in place to autograd, and nothing that it follows is taken."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from neuradar_amd import ops
 
@@ -37,3 +38,22 @@ def test_counters_go_up_for_what_is_written_only():
     before = table._version, grad._version
     ops.embedding_grad(grad, idx, 6, out=table)
     assert table._version > before[0] and grad._version == before[1]
+
+
+def test_followed_tensors_are_refused():
+    leaf, plain, idx = torch.randn(3, 2, device=DEV, requires_grad=True), torch.randn(3, 2, device=DEV), torch.tensor([0, 1, 1], device=DEV)
+    kept = plain.clone()
+    calls = [lambda x: ops.grad_norm([plain, x]), lambda x: ops.clip_factor([plain, x], 1.0), lambda x: ops.clip_grads([plain, x], 1.0),
+             lambda x: ops.clip_grads([x], 1.0, out=[plain]), lambda x: ops.clip_grads([plain], 1.0, out=[x]), lambda x: ops.embedding_grad(x, idx, 4),
+             lambda x: ops.embedding_grad(plain, idx, 3, out=x)]
+    for call in calls:
+        for x in (leaf, leaf * 2.0):
+            with pytest.raises(RuntimeError, match="derivative"):
+                call(x)
+        with forward_ad.dual_level(), pytest.raises(RuntimeError, match="derivative"):
+            call(forward_ad.make_dual(plain.clone(), torch.ones(3, 2, device=DEV)))
+    assert torch.equal(plain, kept)
+    with torch.no_grad():
+        assert float(ops.grad_norm([leaf])) > 0.0 and ops.embedding_grad(leaf, idx, 4).shape == (4, 2)
+    with forward_ad.dual_level(), pytest.raises(NotImplementedError):
+        ops.embedding(forward_ad.make_dual(plain.clone(), torch.ones(3, 2, device=DEV)), idx)
