@@ -980,7 +980,9 @@ int nr_adam_hyper(float* step_t, float* dev_hyper, float lr, float lr_final, int
  *   nr_grad_norm    result[0] = (sum x^2)^(1/2) (norm_type 2), sum |x| (1) or max |x| (0) over all elements, sums in fp64 in a fixed
  *                   order; result[1] = min(1, max_norm / (result[0] + 1e-6)), NaN if the norm is.  max_norm >= 0 (infinity: a
  *                   factor of 1).  NaN and infinities of the gradients reach the norm.  No elements: norm 0.
- *   nr_grad_scale   outs[t] = round(result[1] * grads[t]); outs[t] == grads[t] is in place, and then a factor of 1 moves nothing
+ *   nr_grad_scale   outs[t] = round(result[1] * grads[t]); outs[t] == grads[t] of the same type is in place (NR_EINVAL: of another
+ *                   one), and then a factor of 1 moves nothing.  Otherwise no outs[t] may share memory with a gradient or with
+ *                   another outs[u] (not looked for).
  *   nr_grad_clip    nr_grad_norm and nr_grad_scale in one call (the same results; one launch less for short lists)
  *   workspace       nr_grad_norm_workspace_bytes(numel, count) bytes, 8-byte aligned
  * nr_adam_step_clipped: nr_adam_step with the gradient multiplied by clip[0] (device float; result + 1 of nr_grad_norm) besides

@@ -289,6 +289,14 @@ bool list_ok(const void* const* in, const int64_t* numel, const int32_t* dtype, 
   return true;
 }
 
+// A tensor in place is scaled in its own type: as another one, blocks would write what others have not read yet.
+bool places_ok(const void* const* grads, void* const* outs, const int64_t* numel, const int32_t* dtypes, const int32_t* out_dtypes, int count) {
+  if (!list_ok(grads, numel, dtypes, count) || !list_ok(outs, numel, out_dtypes, count)) return false;
+  for (int t = 0; t < count; ++t)
+    if (numel[t] > 0 && grads[t] == outs[t] && dtypes[t] != out_dtypes[t]) return false;
+  return true;
+}
+
 template <int KIND>
 int run_partials(const void* const* in, const int64_t* numel, const int32_t* dtype, int count, const Cut& c, double* partial, hipStream_t stream) {
   return for_each_run(in, nullptr, numel, dtype, nullptr, count, c, [&](const List& l, uint32_t blocks, int64_t before) {
@@ -363,15 +371,15 @@ extern "C" int nr_grad_norm(const void* const* grads, const int64_t* numel, cons
 extern "C" int nr_grad_scale(const void* const* grads, void* const* outs, const int64_t* numel, const int32_t* dtypes, const int32_t* out_dtypes,
                              int count, const float* result, nr_stream_t stream) {
   Cut c;
-  if (!cut_list(numel, count, &c) || !list_ok(grads, numel, dtypes, count) || !list_ok(outs, numel, out_dtypes, count) || result == nullptr)
-    return NR_EINVAL;
+  if (!cut_list(numel, count, &c) || !places_ok(grads, outs, numel, dtypes, out_dtypes, count) || result == nullptr) return NR_EINVAL;
   return run_scale(grads, outs, numel, dtypes, out_dtypes, count, c, result, nr_s(stream));
 }
 
 extern "C" int nr_grad_clip(const void* const* grads, void* const* outs, const int64_t* numel, const int32_t* dtypes, const int32_t* out_dtypes,
                             int count, int norm_type, double max_norm, float* result, void* workspace, nr_stream_t stream) {
   Cut c;
-  if (!norm_args_ok(grads, numel, dtypes, count, norm_type, max_norm, result, workspace, &c) || !list_ok(outs, numel, out_dtypes, count))
+  if (!norm_args_ok(grads, numel, dtypes, count, norm_type, max_norm, result, workspace, &c) ||
+      !places_ok(grads, outs, numel, dtypes, out_dtypes, count))
     return NR_EINVAL;
   auto run = norm_type == kNormMax ? run_clip<kNormMax> : norm_type == kNormSum ? run_clip<kNormSum> : run_clip<kNormTwo>;
   return run(grads, outs, numel, dtypes, out_dtypes, count, c, max_norm, result, static_cast<double*>(workspace), nr_s(stream));

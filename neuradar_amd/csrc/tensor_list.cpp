@@ -60,15 +60,47 @@ extern "C" int nr_mark_written(PyObject* list) {
   }
 }
 
-// 1 if two of the non-empty tensors start at the same address.
-extern "C" int nr_same_address(const int64_t* ptr, int64_t n) {
+namespace {
+struct Range {
+  uint64_t from, to;
+  bool operator<(const Range& o) const { return from < o.from; }
+};
+Range range_of(const int64_t* ptr, const int64_t* numel, const int32_t* dtype, int64_t i) {
+  const uint64_t from = (uint64_t)ptr[i];
+  return {from, from + (uint64_t)numel[i] * (dtype[i] == 0 ? 4 : 2)};
+}
+enum { kApart = 0, kWrittenTwice = 1, kWrittenAndRead = 2 };
+}  // namespace
+
+// Whether writing dst[0 .. n) while src[0 .. n) is read depends on who comes first: kWrittenTwice if two of dst share memory,
+// kWrittenAndRead if one of dst shares memory with one of src and is not that one itself, with its type, at the same place of the
+// list (in place: every element is read and written by one thread).  Empty tensors share nothing.
+extern "C" int nr_shared_memory(const int64_t* src, const int32_t* src_dtype, const int64_t* dst, const int32_t* dst_dtype, const int64_t* numel,
+                                int64_t n) {
   try {
-    std::vector<int64_t> p;
-    p.reserve((size_t)n);
-    for (int64_t i = 0; i < n; ++i)
-      if (ptr[i] != 0) p.push_back(ptr[i]);
-    std::sort(p.begin(), p.end());
-    return std::adjacent_find(p.begin(), p.end()) != p.end() ? 1 : 0;
+    std::vector<Range> out;
+    out.reserve((size_t)n);
+    uint64_t low = UINT64_MAX, high = 0;  // (of src, without what is in place)
+    for (int64_t i = 0; i < n; ++i) {
+      if (numel[i] <= 0) continue;
+      out.push_back(range_of(dst, numel, dst_dtype, i));
+      if (src[i] == dst[i] && src_dtype[i] == dst_dtype[i]) continue;
+      const Range r = range_of(src, numel, src_dtype, i);
+      low = std::min(low, r.from);
+      high = std::max(high, r.to);
+    }
+    if (out.empty()) return kApart;
+    if (!std::is_sorted(out.begin(), out.end())) std::sort(out.begin(), out.end());
+    for (size_t k = 1; k < out.size(); ++k)
+      if (out[k].from < out[k - 1].to) return kWrittenTwice;
+    if (high <= out.front().from || low >= out.back().to) return kApart;
+    for (int64_t i = 0; i < n; ++i) {  // (the ranges of out are apart, so their ends ascend too: the first that ends behind r's start)
+      if (numel[i] <= 0 || (src[i] == dst[i] && src_dtype[i] == dst_dtype[i])) continue;
+      const Range r = range_of(src, numel, src_dtype, i);
+      const auto at = std::upper_bound(out.begin(), out.end(), r.from, [](uint64_t a, const Range& o) { return a < o.to; });
+      if (at != out.end() && at->from < r.to) return kWrittenAndRead;
+    }
+    return kApart;
   } catch (...) {
     return kFailed;
   }

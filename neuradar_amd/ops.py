@@ -1421,7 +1421,8 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> Tens
     """Scale gradients by min(1, max_norm / (norm + 1e-6)), norm = grad_norm(grads, norm_type), which is returned.  In place, or
     into the tensors of `out` (as many elements each, any of the three types: places in a 16-bit bucket, say), one rounding.
     Nothing is read on the host; a norm of NaN makes every gradient NaN, as in torch.  Tensors that are written must not share
-    memory (two that start at one address are refused).  Not differentiable: tensors that autograd follows are refused (under
+    memory, neither with one another nor with a gradient other than their own in its own type: refused (of tensors with holes, those
+    that start at one address).  Not differentiable: tensors that autograd follows are refused (under
     torch.no_grad() they are not); a graph that saved a tensor which is written here raises when it is differentiated."""
     grads = _as_list(grads)
     targets = grads if out is None else _as_list(out)
@@ -1445,11 +1446,19 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> Tens
                 raise RuntimeError("out must have its gradients' shapes where one of the two is not contiguous")
             src = _GradList([g.contiguous() for g in grads], "gradients")
             dst = _GradList([o if o.is_contiguous() else torch.empty_like(o, memory_format=torch.contiguous_format) for o in targets], "out")
-    if _lib.tensors().nr_same_address(dst.arrays[0], dst.count) != 0:
-        raise RuntimeError("a tensor to be written is listed twice")
+    shared = _lib.tensors().nr_shared_memory(src.arrays[0], src.arrays[2], dst.arrays[0], dst.arrays[2], src.arrays[1], src.count)
+    moved = not dst.plain or dst.tensors is not targets
+    if moved:
+        starts = [t.data_ptr() for t in targets if t.numel() > 0]
+        shared = shared or int(len(set(starts)) < len(starts))
+        if any(s == 0 and n > 1 for t in targets for s, n in zip(t.stride(), t.shape)):
+            raise RuntimeError("a tensor to be written holds several of its elements in one place")
+    if shared != 0:
+        raise RuntimeError("a tensor to be written is listed twice, or shares memory with another" if shared == 1 else
+                           "a tensor to be written shares memory with a gradient (in place it has to be that gradient, in its own type)")
     result = _norm_and_factor(src, float(max_norm), norm_type, device, dst)
     _lib.tensors().nr_mark_written(targets)
-    if not dst.plain or dst.tensors is not targets:
+    if moved:
         for target, written in zip(targets, dst.tensors):  # a target with holes gets its elements from a dense copy
             if written.data_ptr() != target.data_ptr():
                 target.copy_(written)
