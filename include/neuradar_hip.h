@@ -901,7 +901,8 @@ int nr_appearance_concat_bwd(const float* grad_out, int n_channels, int app_dim,
  *   nr_embedding_bwd   grad_table[v, c] = round(scale * sum of grad[i, c] over idx[i] == v), sums in fp32 and rounded once;
  *                      accumulate != 0: round(grad_table[v, c] + that) on the rows looked up, the others untouched; 0: the
  *                      others are zero.  Indices equal to `padding` (-1: none) or outside [0, rows) contribute nothing.
- *                      grad: rows grad_stride >= 0 elements apart (0: one row for all).  grad_table: contiguous.
+ *                      grad: rows grad_stride >= 0 elements apart (0: one row for all).  grad_table: contiguous, no memory
+ *                      shared with grad or idx (not looked for).
  *   workspace          nr_embedding_bwd_workspace_bytes(...) bytes, 256-byte aligned, contents irrelevant before and after
  * dim <= 65 536, rows < 2^31 - 1, n < 2^31 (NR_EINVAL otherwise).  n = 0: nothing is read; a gradient that is not accumulated is
  * all zero.

@@ -751,6 +751,18 @@ def _strided_rows(t: Tensor) -> Tuple[Tensor, int]:
     return t, t.stride(0)
 
 
+def _shares_memory(rows: Tensor, stride: int, out: Tensor) -> bool:
+    """Whether a contiguous `out` has a byte of `rows` [n, dim], which lie `stride` elements apart (between them it may lie)."""
+    n, size = rows.shape[0], rows.element_size()
+    step, row = stride * size, rows.shape[1] * size
+    lo = out.data_ptr() - rows.data_ptr()  # out's bytes, from the first row's start on
+    hi = lo + out.numel() * out.element_size()
+    if n == 0 or row == 0 or lo == hi:
+        return False
+    first = 0 if lo < row or step == 0 else (lo - row) // step + 1  # the first row that ends behind out's start
+    return first < n and first * step < hi and first * step + row > lo
+
+
 def _embedding_rows(table: Tensor, idx: Tensor, scale: float) -> Tensor:
     device = table.get_device()
     if device != _current_device():
@@ -794,9 +806,9 @@ def embedding_grad(grad: Tensor, idx: Tensor, num_rows: int, scale: float = 1.0,
     elif (_float_rows(out, "out").shape != (num_rows, dim) or not out.is_contiguous() or out.get_device() != device
           or dtype not in (None, out.dtype)):
         raise RuntimeError(f"out must be a contiguous [{num_rows}, {dim}] tensor on grad's device" + ("" if dtype is None else f" of {dtype}"))
-    if n > 0 and dim > 0 and out.data_ptr() == grad.data_ptr():
-        raise RuntimeError("out must not be grad")
     grad, stride = _strided_rows(grad)
+    if given and (_shares_memory(grad, stride, out) or _shares_memory(idx.view(1, -1), n, out)):
+        raise RuntimeError("out must not be grad or idx, nor share memory with them")
     code = _DTYPE_CODES[grad.dtype]
     lib = _lib.lib()
     need = lib.nr_embedding_bwd_workspace_bytes(num_rows, dim, n, code)

@@ -1,10 +1,10 @@
-"""CPU (no GPU): what the clipping refuses because it shares memory, on addresses alone."""
+"""CPU (no GPU): what the clipping and the embedding gradient refuse because it shares memory, on addresses alone."""
 from array import array
 
 import pytest
 import torch
 
-from neuradar_amd import _lib
+from neuradar_amd import _lib, ops
 
 BASE = 1 << 30
 F32, BF16, F16 = 0, 1, 2
@@ -62,6 +62,23 @@ def test_lists_against_the_definition():
         assert got == by_bytes(src, dst), (src, dst)
         seen.add(got)
     assert seen == {APART, TWICE, READ}
+
+
+def test_rows_and_a_result():
+    """Rows of a wide buffer against a contiguous place anywhere in it: the bytes of both, compared as sets."""
+    base = torch.arange(240, dtype=torch.float32)
+    cells = lambda t: {t.data_ptr() + 4 * (sum(i * s for i, s in zip(at, t.stride()))) for at in [  # noqa: E731
+        (i, j) for i in range(t.shape[0]) for j in range(t.shape[1])]}
+    found = set()
+    for n, dim, stride, at in ((5, 4, 10, 30), (5, 10, 10, 3), (1, 4, 0, 50), (6, 4, 0, 50), (4, 6, 3, 20), (3, 1, 40, 100), (0, 4, 10, 0), (3, 0, 10, 0)):
+        rows = base.as_strided((n, dim), (stride, 1), at)
+        for place in range(0, 200, 1):
+            for shape in ((1, 3), (2, 3), (1, 0), (3, 13)):
+                out = base[place:place + shape[0] * shape[1]].view(shape)
+                want = bool(cells(rows) & cells(out))
+                assert ops._shares_memory(rows, stride, out) == want, (n, dim, stride, at, place, shape)
+                found.add(want)
+    assert found == {True, False}
 
 
 def test_c_entry_points_refuse_in_place_in_another_type():

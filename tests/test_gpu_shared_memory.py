@@ -39,3 +39,22 @@ def test_clipping_beside_and_in_place():
     assert torch.allclose(halves, want, rtol=2.0 ** -21, atol=0)
     empty = torch.empty(0, device=DEV)
     assert float(ops.clip_grads([empty, empty], 1.0)) == 0.0
+
+
+def test_embedding_gradient_refuses_shared_memory():
+    idx = torch.tensor([0, 1, 1, 3], device=DEV)
+    buf = torch.randn(4 * 20, device=DEV)
+    kept = buf.clone()
+    wide = buf.view(4, 20)
+    grad = wide[:, :8]
+    for out in (buf[:32].view(4, 8), buf[30:62].view(4, 8), buf[40:72].view(4, 8), buf.view(BF16)[:32].view(4, 8)):
+        for accumulate in (False, True):
+            with pytest.raises(RuntimeError, match="share memory"):
+                ops.embedding_grad(grad, idx, 4, out=out, accumulate=accumulate)
+    with pytest.raises(RuntimeError, match="share memory"):
+        ops.embedding_grad(torch.ones(4, 1, device=DEV), idx, 8, out=idx.view(torch.float32).view(8, 1))
+    assert torch.equal(buf, kept)
+    room = buf[8:16].view(1, 8)  # between two rows of grad
+    want = (grad[idx == 0].sum(0), wide[1:].clone())
+    ops.embedding_grad(grad, idx, 1, out=room)
+    assert torch.equal(room[0], want[0]) and torch.equal(wide[1:], want[1]) and torch.equal(wide[0, :8], kept[:8])
