@@ -6,7 +6,8 @@
 // tensor happens to be the last block of its segment -- which depends on everything the process allocated before (the round-4
 // suite aborted in 2 of 8 runs, no test alone ever did).  Here every allocation is its own hipMalloc'ed region, rounded up to a
 // multiple of 2 MB, and the tensor is its LAST bytes (start rounded down to 16 bytes: vector accesses stay aligned).  The runtime
-// spaces such regions 2 MB apart with nothing mapped in between (tools/probe_redzone.py: an overrun of 8 bytes faults).
+// spaces such regions 2 MB apart with nothing mapped in between (observed: 8 bytes behind a region's end faulted).  guard_layout is
+// the arithmetic alone, for a test on the host.
 // 64 canary bytes in front of every tensor are checked when it is freed (writes before the start): guard_canary_failures().
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -25,11 +26,18 @@ std::unordered_map<void*, void*> g_base;  // tensor address -> region base
 long g_failures = 0, g_allocs = 0;
 }  // namespace
 
+// A tensor of `size` bytes: *region bytes to allocate, the tensor at *offset in them, *span of them its own (to the region's end).
+extern "C" void guard_layout(size_t size, size_t* region, size_t* offset, size_t* span) {
+  *span = (size + 15) & ~(size_t)15;
+  *region = (*span + kCanary + kGranule - 1) / kGranule * kGranule;
+  *offset = *region - *span;
+}
+
 extern "C" void* guard_malloc(ssize_t size, int device, hipStream_t stream) {
   (void)stream;
   if (size <= 0) size = 1;
-  const size_t span = ((size_t)size + 15) & ~(size_t)15;
-  const size_t region = (span + kCanary + kGranule - 1) / kGranule * kGranule;
+  size_t region, offset, span;
+  guard_layout((size_t)size, &region, &offset, &span);
   int prev = 0;
   hipGetDevice(&prev);
   if (prev != device) hipSetDevice(device);
@@ -38,7 +46,7 @@ extern "C" void* guard_malloc(ssize_t size, int device, hipStream_t stream) {
     if (prev != device) hipSetDevice(prev);
     return nullptr;
   }
-  char* p = static_cast<char*>(base) + region - span;
+  char* p = static_cast<char*>(base) + offset;
   hipMemset(p - kCanary, 0xA5, kCanary);  // (synchronous enough: the null stream orders it in front of later work)
   if (prev != device) hipSetDevice(prev);
   std::lock_guard<std::mutex> lock(g_mutex);
