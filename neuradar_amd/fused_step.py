@@ -958,6 +958,11 @@ class FusedTrainStep:
                 reducer.wait_all()  # stream-level wait: the stream continues once RCCL is done
             table_opt.step_buffer(i_prop, scale)
 
+        def never_evaluated():
+            """Addresses of proposal_fields[:-1]'s parameters (the reference's late-binding lambda evaluates the last field only,
+            neuradar.py:302): their gradient is identically zero."""
+            return {p_.data_ptr() for f_ in self.model.proposal_fields[:-1] for p_ in f_.parameters()}
+
         def small_and_other_steps():
             if reducer is not None:  # small parameters: need field_bwd and both prop_density_bwd
                 for _, g_ in field_opt.buffers:
@@ -967,9 +972,8 @@ class FusedTrainStep:
                 field_opt.check_buffer(i)  # (loss scaler attached: found-inf of the small parameters' gradients)
                 field_opt.step_buffer(i, scale)
             # whatever else the table optimizer holds (per-actor grids) and the trajectory optimizer
-            # ... except the tables of proposal_fields[:-1]: never evaluated (the reference's late-binding lambda,
-            # neuradar.py:302), so their gradient is identically zero -- neither all-reduced nor walked by Adam
-            dead = {p_.data_ptr() for f_ in self.model.proposal_fields[:-1] for p_ in f_.parameters()}
+            # ... except the never evaluated ones, neither all-reduced nor walked by Adam
+            dead = never_evaluated()
             others = [(table_opt, i) for i in range(len(table_opt.buffers))
                       if i not in (i_prop, i_main) and table_opt.buffers[i][0].data_ptr() not in dead]
             others += [(o_, i) for o_ in optimizers[2:] for i in range(len(o_.buffers))]
@@ -1057,7 +1061,7 @@ class FusedTrainStep:
                 if o_ is not behind[0]:
                     for i in range(len(o_.buffers)):
                         o_.check_buffer(i)  # (the tables' gradients are flagged by the field backward)
-                o_.step()
+                o_.step(leave=never_evaluated() if o_ is behind[0] else ())
             if self.amp is not None:
                 self.amp.update()
         return self.loss

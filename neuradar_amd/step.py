@@ -777,7 +777,8 @@ class FlatAdam:
         raise KeyError("parameter is not managed by this optimizer")
 
     @torch.no_grad()
-    def step(self) -> None:
+    def step(self, leave=()) -> None:
+        """One step on every buffer.  leave: addresses of buffers that are not stepped (no gradient: no weight decay either)."""
         self.advance()
         if hasattr(self, "marked"):  # whoever calls step() wrote the gradients without marking `seen` (modular backward, a
             self.marked.clear()      # collective): only FusedTrainStep pairs its marking scatter with step_buffer()
@@ -785,4 +786,5 @@ class FlatAdam:
         if self.max_norm is not None:
             self.total_norm, clip = ops.clip_factor(self.grad_buffers(), self.max_norm)
         for i in range(len(self.buffers)):
-            self.step_buffer(i, clip=clip)
+            if self.buffers[i][0].data_ptr() not in leave:
+                self.step_buffer(i, clip=clip)

@@ -1,0 +1,84 @@
+"""GPU: FusedTrainStep with optimizers that clip (max_norm), beside what else steps differ in: the device-resident loss scaler, tables that
+the step never evaluates."""
+import math
+
+import pytest
+import torch
+
+from helpers import load_golden
+from test_gpu_amp import _fp16_step, _snapshot
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def moments(opt):
+    return [m.reshape(-1).double().clone() for m, _ in opt.state]
+
+
+def norm_of(ms):
+    return math.sqrt(sum(float((m / 0.1).square().sum()) for m in ms))  # (the first step's exp_avg is 0.1 times the gradient)
+
+
+def test_the_loss_scaler_and_clipping_together():
+    """A clipped fp16 step's first moments are the factor times those of the step that does not clip, whatever the loss scale is (the
+    norm is of the gradients without it).  Tolerance: two runs of the step differ by the order of float atomics and, where that
+    moves an fp16 operand across a rounding border, by 2^-11 of an addend: 1e-2 of a buffer's largest entry is ten times that."""
+    model, opts, fused, amp, args, rnd, tf, td = _fp16_step()
+    fused.forward_backward(*args, tf, td, *rnd, optimizers=opts)
+    plain = [moments(o) for o in opts]
+    norms = [norm_of(ms) for ms in plain]
+    for ratios in ((0.25, None), (None, 0.5), (0.25, 0.5), (4.0, 4.0)):
+        model, opts, fused, amp, args, rnd, tf, td = _fp16_step()
+        for opt, ratio, norm in zip(opts, ratios, norms):
+            opt.max_norm = None if ratio is None else ratio * norm
+        loss = fused.forward_backward(*args, tf, td, *rnd, optimizers=opts)
+        assert math.isfinite(float(loss.sum())) and amp.skipped_steps() == 0
+        for opt, ratio, norm, want in zip(opts, ratios, norms, plain):
+            factor = 1.0 if ratio is None else min(1.0, ratio)
+            if ratio is not None:
+                assert abs(float(opt.total_norm) - norm) <= 1e-2 * norm
+            for m, w in zip(moments(opt), want):
+                assert float((m - factor * w).abs().max()) <= 1e-2 * factor * float(w.abs().max()) + 1e-12
+            assert not any(bool(g.any()) for g in opt.grad_buffers())
+
+
+def test_an_overflow_is_skipped_with_clipping_too():
+    """An overflowed step moves nothing, whatever its norm is (infinite or NaN, and with it the factor); the next one trains."""
+    model, opts, fused, amp, args, rnd, tf, td = _fp16_step()
+    for opt in opts:
+        opt.max_norm = 1e-3
+    fused.forward_backward(*args, tf, td, *rnd, optimizers=opts)
+    before, scale = _snapshot(model, opts), amp.get_scale()
+    fused.forward_backward(*args, torch.full_like(tf, 1e30), td, *rnd, optimizers=opts)
+    after = _snapshot(model, opts)
+    for key in before:
+        assert "seen" in key or torch.equal(before[key], after[key]), key
+    assert amp.skipped_steps() == 1 and amp.get_scale() == 0.5 * scale
+    assert all(not bool(g.any()) for opt in opts for g in opt.grad_buffers())
+    fused.forward_backward(*args, tf, td, *rnd, optimizers=opts)
+    again = _snapshot(model, opts)
+    assert any(not torch.equal(after[k], again[k]) for k in after) and all(bool(torch.isfinite(v.float()).all()) for v in again.values())
+    assert amp.skipped_steps() == 1 and all(math.isfinite(float(o.total_norm)) for o in opts)
+
+
+@pytest.mark.parametrize("max_norm", [None, 1e9])
+def test_tables_that_are_never_evaluated_are_left_alone(max_norm):
+    """proposal_fields[0] is never evaluated: its table gets no gradient and, like a parameter whose .grad is None, no weight decay."""
+    from neuradar_amd.fused_step import FusedTrainStep
+    from neuradar_amd.step import FlatAdam
+    from test_gpu_parity import build_hot_path, dev
+
+    g = load_golden("pipeline")
+    model = build_hot_path(g).train()
+    groups = model.get_param_groups()
+    table = model.proposal_fields[0].hashgrid.static_grid.hash_table
+    opts = [FlatAdam(groups["hashgrids"], lr=1e-2, warmup_steps=0, weight_decay=0.1, adamw=True, flatten=False, max_norm=max_norm),
+            FlatAdam(groups["fields"], lr=1e-2, warmup_steps=0, skip=list(model.proposal_fields[0].parameters()))]
+    assert any(b.data_ptr() == table.data_ptr() for b, _ in opts[0].buffers)
+    before, other = table.detach().clone(), model.field.hashgrid.static_grid.hash_table.detach().clone()
+    fused = FusedTrainStep(model, g["origins"].shape[0])
+    fused.forward_backward(dev(g["origins"]), dev(g["directions"]), dev(g["pixel_area"])[:, 0].contiguous(), dev(g["fars"])[:, 0].contiguous(),
+                           dev(g["target_features"]), dev(g["target_depth"])[:, 0].contiguous(), dev(g["t_rand"]), dev(g["jitter1"])[:, 0].contiguous(),
+                           dev(g["jitter2"])[:, 0].contiguous(), optimizers=opts)
+    assert torch.equal(table, before) and not torch.equal(model.field.hashgrid.static_grid.hash_table, other)
