@@ -62,6 +62,42 @@ def test_an_overflow_is_skipped_with_clipping_too():
     assert amp.skipped_steps() == 1 and all(math.isfinite(float(o.total_norm)) for o in opts)
 
 
+def test_a_clipped_fused_step_replays_as_a_graph():
+    """Four steps, eager and replayed, with an eps above the gradients (so that Adam is smooth in them): what the two runs' parameters
+    moved by differs by the order of the step's float atomics only, an fp16 rounding of an addend at most."""
+    def make():
+        model, opts, fused, amp, args, rnd, tf, td = _fp16_step()
+        for opt in opts:
+            opt.max_norm, opt.eps, opt.wd = 1e-2, 1.0, 0.0
+        start = {n: p.detach().clone() for n, p in model.named_parameters()}
+        return model, opts, amp, start, lambda: fused.forward_backward(*args, tf, td, *rnd, optimizers=opts)
+
+    (ma, oa, _, start, step_a), (mb, ob, amp, _, step_b) = make(), make()
+    norms = []
+    for _ in range(5):
+        step_a()
+        norms.append([float(o.total_norm) for o in oa])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step_b()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            step_b()
+        for k in range(1, 5):
+            graph.replay()
+            torch.cuda.synchronize()
+            for o, want in zip(ob, norms[k]):
+                assert abs(float(o.total_norm) - want) <= 1e-2 * want
+    torch.cuda.current_stream().wait_stream(side)
+    assert amp.skipped_steps() == 0
+    for (n, p), q in zip(ma.named_parameters(), mb.parameters()):
+        moved = float((p.detach().double() - start[n].double()).norm())
+        if moved > 0.0:
+            assert float((p.detach().double() - q.detach().double()).norm()) <= 2e-2 * moved, n
+
+
 @pytest.mark.parametrize("max_norm", [None, 1e9])
 def test_tables_that_are_never_evaluated_are_left_alone(max_norm):
     """proposal_fields[0] is never evaluated: its table gets no gradient and, like a parameter whose .grad is None, no weight decay."""
