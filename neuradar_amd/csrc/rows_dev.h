@@ -1,6 +1,8 @@
 // Element types and unaligned vector access of the kernels that take fp32, bf16 and fp16 tensors of any alignment
 // (embedding.hip, grad_norm.hip).
 #pragma once
+#include <type_traits>
+
 #include "nr_common.h"
 
 namespace {
@@ -19,12 +21,19 @@ __device__ __forceinline__ void nr_load_pack(const T* __restrict__ p, float (&x)
 #pragma unroll
   for (int k = 0; k < N; ++k) x[k] = (float)v[k];
 }
-// one rounding to T (to nearest even), of a value held in fp32
+// One rounding to T (to nearest even) of a value held in fp32.  The compiler may form a product and round it to fp16 in one instruction
+// (v_fma_mixlo_f16: once, not first to fp32), and does so in some loops and not in others: an element's bits would depend on where in
+// its tensor it lies.  So the value is taken as it stands in its register.
+template <typename T>
+__device__ __forceinline__ T nr_round(float x) {
+  if constexpr (std::is_same_v<T, _Float16>) asm("" : "+v"(x));
+  return (T)x;
+}
 template <typename T, int N>
 __device__ __forceinline__ void nr_store_pack(T* __restrict__ p, const float (&x)[N]) {
   typename NrPack<T, N>::vec v;
 #pragma unroll
-  for (int k = 0; k < N; ++k) v[k] = (T)x[k];
+  for (int k = 0; k < N; ++k) v[k] = nr_round<T>(x[k]);
   reinterpret_cast<NrPack<T, N>*>(p)->v = v;
 }
 // the same without a place in the caches, for results that are larger than those: what they would push out is read again
@@ -32,7 +41,7 @@ template <typename T, int N>
 __device__ __forceinline__ void nr_store_pack_stream(T* __restrict__ p, const float (&x)[N]) {
   typename NrPack<T, N>::vec v;
 #pragma unroll
-  for (int k = 0; k < N; ++k) v[k] = (T)x[k];
+  for (int k = 0; k < N; ++k) v[k] = nr_round<T>(x[k]);
   __builtin_nontemporal_store(v, reinterpret_cast<typename NrPack<T, N>::vec*>(p));
 }
 // Results beyond this size leave through nr_store_pack_stream: the 256 MB cache in front of the memory cannot hold them for
@@ -107,7 +116,7 @@ __device__ __forceinline__ void nr_store_some(T* __restrict__ p, int m, const fl
   typedef T whole __attribute__((ext_vector_type(16 / sizeof(T))));
   whole v = {};
 #pragma unroll
-  for (int k = 0; k < N && k < (int)(16 / sizeof(T)); ++k) v[k] = (T)x[k];
+  for (int k = 0; k < N && k < (int)(16 / sizeof(T)); ++k) v[k] = nr_round<T>(x[k]);
   const two64 all = __builtin_bit_cast(two64, v);
   const int bytes = m * (int)sizeof(T);
   char* at = reinterpret_cast<char*>(p);
