@@ -898,7 +898,9 @@ int nr_appearance_concat_bwd(const float* grad_out, int n_channels, int app_dim,
  *   idx       [n] int32 (idx_bytes 4) or int64 (8)
  *   nr_embedding_fwd   out[i*out_stride + c] = round(scale * table[idx[i], c]); an index outside [0, rows) reads nothing and
  *                      gives a row of NaN
- *   nr_embedding_bwd   grad_table[v, c] = round(scale * sum of grad[i, c] over idx[i] == v), sums in fp32 and rounded once;
+ *   nr_embedding_bwd   grad_table[v, c] = round(scale * sum of grad[i, c] over idx[i] == v); sums in 64 bits, rounded to fp32
+ *                      where they pass through the workspace and, for 16-bit grad, between a block's groups of lanes (up to
+ *                      12 times); the product with scale is rounded to fp32, then to the table's type.
  *                      accumulate != 0: round(grad_table[v, c] + that) on the rows looked up, the others untouched; 0: the
  *                      others are zero.  Indices equal to `padding` (-1: none) or outside [0, rows) contribute nothing.
  *                      grad: rows grad_stride >= 0 elements apart (0: one row for all).  grad_table: contiguous, no memory

@@ -6,8 +6,9 @@
 // The gradient is a sum over equal indices.  Adding rows to the table as they come needs float atomics, whose order -- and with
 // it the result -- changes from run to run, and a row that many tokens share becomes one queue at the memory side.  Here equal
 // indices are brought together first, their positions in ascending order; then every sum is formed in registers in one fixed
-// order and each touched row is written once.  All sums are held in fp32; the order follows from (n, rows, dim, type) alone: two
-// calls give the same bits.  Three ways, by sizes (make_own_plan, make_plan):
+// order and each touched row is written once.  Sums are held in 64 bits inside a block and in fp32 in the workspace; their order
+// follows from the sizes, the types and the indices alone: two calls give the same bits.  Three ways, by sizes (make_own_plan,
+// make_plan):
 //   * up to 16 384 indices, one launch: a block owns a range of rows, picks its tokens out of all indices and orders them in LDS
 //     (own_kernel);
 //   * more indices and a table whose copies are small: the same on chunks of the indices, and a launch that adds the chunks' tables;
@@ -21,6 +22,8 @@
 // a cold table); gradient 16 384 x 16 on 60 rows 11 us, 113 840 x 32 on 1 999 rows 18 + 4, 8 192 x 8 on 2^22 rows 25 (134 MB of
 // zeros alone: 18), 100 003 x 257 on 7 rows 32 + 4 (103 MB: 20), 131 072 x 512 bf16 on 131 072 rows 108 (sort 45, which also
 // writes the zeros; sums 53 at 3.2 TB/s; join 9).
+#include <type_traits>
+
 #include "rows_dev.h"
 
 namespace {
@@ -291,24 +294,68 @@ struct SumArgs {
 };
 constexpr uint32_t kHead = 1u, kSpan = 2u, kTail = 4u;
 
-template <int N, typename O>
-__device__ __forceinline__ void write_row_as(const SumArgs& a, uint32_t row, int col, float (&x)[N]) {
-  O* o = static_cast<O*>(a.out) + (int64_t)row * a.dim + col;
+// A sum is held in 64 bits while it is in registers, and between the groups of a block where 4 columns make a vector (fp32 rows).  14 000
+// addends a row: off by 3.5e-8 of the largest (the result's own rounding alone: 2.5e-8), 1.4e-7 with all of it in fp32, which takes 1.1 us
+// less of the kernel's 33 (113 840 tokens on 1 999 rows: 2.8e-8 and 8.7e-8, 1.2 of 19).  It is rounded to fp32 where it goes to the
+// workspace, and between the groups where 8 columns make a vector, whose 64 bits would not fit beside a full list of tokens (16-bit
+// rows; 2^-24 of a sum of 16-bit values).
+template <int N>
+using Part = std::conditional_t<N == 4, double, float>;
+
+template <int N>
+__device__ __forceinline__ void part_get(const Part<N>* p, double (&x)[N]) {
+  typedef Part<N> vec __attribute__((ext_vector_type(16 / sizeof(Part<N>))));
+  constexpr int M = 16 / (int)sizeof(Part<N>);
 #pragma unroll
-  for (int k = 0; k < N; ++k) x[k] *= a.scale;
-  if (a.accumulate) {
-    float was[N];
-    nr_load_some<O, N>(o, a.dim - col, was);
+  for (int q = 0; q < N / M; ++q) {
+    const vec v = reinterpret_cast<const vec*>(p)[q];
 #pragma unroll
-    for (int k = 0; k < N; ++k) x[k] += was[k];
+    for (int k = 0; k < M; ++k) x[q * M + k] = (double)v[k];
   }
-  nr_store_some<O, N>(o, a.dim - col, x);
 }
 template <int N>
-__device__ __forceinline__ void write_row(const SumArgs& a, uint32_t row, int col, float (&x)[N]) {
-  if (a.out_dtype == NR_DTYPE_F32) write_row_as<N, float>(a, row, col, x);
-  else if (a.out_dtype == NR_DTYPE_BF16) write_row_as<N, __bf16>(a, row, col, x);
-  else write_row_as<N, _Float16>(a, row, col, x);
+__device__ __forceinline__ void part_put(Part<N>* p, const double (&x)[N]) {
+  typedef Part<N> vec __attribute__((ext_vector_type(16 / sizeof(Part<N>))));
+  constexpr int M = 16 / (int)sizeof(Part<N>);
+#pragma unroll
+  for (int q = 0; q < N / M; ++q) {
+    vec v;
+#pragma unroll
+    for (int k = 0; k < M; ++k) v[k] = (Part<N>)x[q * M + k];
+    reinterpret_cast<vec*>(p)[q] = v;
+  }
+}
+
+// The first `m` columns of a sum to the workspace.
+template <int N>
+__device__ __forceinline__ void leave(float* p, int m, const double (&x)[N]) {
+  float y[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) y[k] = (float)x[k];
+  nr_store_some<float, N>(p, m, y);
+}
+
+// o (+)= y, the first `m` columns
+template <int N, typename O>
+__device__ __forceinline__ void write_as(O* o, int m, bool accumulate, float (&y)[N]) {
+  if (accumulate) {
+    float was[N];
+    nr_load_some<O, N>(o, m, was);
+#pragma unroll
+    for (int k = 0; k < N; ++k) y[k] += was[k];
+  }
+  nr_store_some<O, N>(o, m, y);
+}
+template <int N>
+__device__ __forceinline__ void write_row(const SumArgs& a, uint32_t row, int col, const double (&x)[N]) {
+  const int64_t at = (int64_t)row * a.dim + col;
+  const int m = a.dim - col;
+  float y[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) y[k] = (float)(x[k] * (double)a.scale);
+  if (a.out_dtype == NR_DTYPE_F32) write_as<N, float>(static_cast<float*>(a.out) + at, m, a.accumulate != 0, y);
+  else if (a.out_dtype == NR_DTYPE_BF16) write_as<N, __bf16>(static_cast<__bf16*>(a.out) + at, m, a.accumulate != 0, y);
+  else write_as<N, _Float16>(static_cast<_Float16*>(a.out) + at, m, a.accumulate != 0, y);
 }
 
 constexpr int kMaxStretch = 4096;  // sorted positions of one block (32 KB of LDS)
@@ -322,13 +369,13 @@ constexpr int kFlight = 8;         // rows of g requested before the first of th
 // (131 072 x 513 bf16: 141 -> 119 us against pieces, whose branches keep the rows of a flight from being requested together).
 template <typename T, int N, typename Key, typename Pos>
 __device__ __forceinline__ uint32_t walk_stretch(const SumArgs& a, const T* __restrict__ grad, int q0, int q1, int col, uint32_t row0, Key key_at,
-                                                 Pos pos_at, float* head, float* tail) {
+                                                 Pos pos_at, Part<N>* head, Part<N>* tail) {
   uint32_t flag = 0u;
   const int back = a.dim >= N ? max(col + N - a.dim, 0) : 0;
   const T* from = grad + (col - back);
-  float acc[N];
+  double acc[N];
 #pragma unroll
-  for (int k = 0; k < N; ++k) acc[k] = 0.0f;
+  for (int k = 0; k < N; ++k) acc[k] = 0.0;
   uint32_t key[kFlight + 1];
   key[kFlight] = key_at(q0);
   bool open_here = key_at(q0 - 1) != key[kFlight];
@@ -354,7 +401,7 @@ __device__ __forceinline__ uint32_t walk_stretch(const SumArgs& a, const T* __re
       if (q + u >= q1) break;
       const bool goes_on = key[u] == key[u + 1];
 #pragma unroll
-      for (int k = 0; k < N; ++k) acc[k] += x[u][k];
+      for (int k = 0; k < N; ++k) acc[k] += (double)x[u][k];
       if (goes_on && q + u + 1 < q1) continue;
 #pragma unroll
       for (int step = 1; step < N; step *= 2) {
@@ -362,7 +409,7 @@ __device__ __forceinline__ uint32_t walk_stretch(const SumArgs& a, const T* __re
 #pragma unroll
         for (int k = 0; k + step < N; ++k) acc[k] = acc[k + step];
       }
-      float* part = nullptr;
+      Part<N>* part = nullptr;
       if (!open_here) {
         part = head;
         flag |= goes_on ? kHead | kSpan : kHead;
@@ -371,13 +418,13 @@ __device__ __forceinline__ uint32_t walk_stretch(const SumArgs& a, const T* __re
         flag |= kTail;
       }
       if (part != nullptr) {
-        nr_lds_put<N>(part, acc);
+        part_put<N>(part, acc);
       } else {
         write_row<N>(a, row0 + key[u], col, acc);
       }
       open_here = true;
 #pragma unroll
-      for (int k = 0; k < N; ++k) acc[k] = 0.0f;
+      for (int k = 0; k < N; ++k) acc[k] = 0.0;
     }
   }
   return flag;
@@ -407,22 +454,22 @@ __device__ __forceinline__ int first_stop(const uint64_t* span, int g, int group
 // threads call it, behind a barrier; `used`: groups with tokens; `head`: this thread's columns of group 0.  A group's own sum stays
 // in registers and its columns move as 16-byte vectors (3 822 tokens on one row of 8 fp16 values: 11.6 us of the kernel -> 3.9).
 template <int N>
-__device__ __forceinline__ void chain_heads(const uint64_t* span, int r, bool work, int groups, int used, float* head, int step) {
+__device__ __forceinline__ void chain_heads(const uint64_t* span, int r, bool work, int groups, int used, Part<N>* head, int step) {
   uint64_t any = 0ull;
   for (int w = 0; w * NR_WAVE < groups; ++w) any |= span[w];
   if (any == 0ull) return;
   const int run = work ? first_stop(span, r, groups) - r : 0;  // groups from r on that hand on
-  float* at = head + r * step;
-  float own[N] = {}, x[N];
-  if (run > 0) nr_lds_get<N>(at, own);
+  Part<N>* at = head + r * step;
+  double own[N] = {}, x[N];
+  if (run > 0) part_get<N>(at, own);
   for (int d = 1; d < used; d *= 2) {
     const bool add = run >= d && r + d < groups;
-    if (add) nr_lds_get<N>(at + d * step, x);
+    if (add) part_get<N>(at + d * step, x);
     __syncthreads();
     if (add) {
 #pragma unroll
       for (int k = 0; k < N; ++k) own[k] += x[k];
-      nr_lds_put<N>(at, own);
+      part_put<N>(at, own);
     }
     __syncthreads();
   }
@@ -434,8 +481,8 @@ sum_kernel(SumArgs a, const T* __restrict__ grad) {
   constexpr int N = 16 / (int)sizeof(T);
   extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
   const int per_block = a.groups * a.per_group, step = a.group * N;
-  float* s_head = reinterpret_cast<float*>(lds);    // [groups][group * N]
-  float* s_tail = s_head + a.groups * step;
+  Part<N>* s_head = reinterpret_cast<Part<N>*>(lds);  // [groups][group * N]
+  Part<N>* s_tail = s_head + a.groups * step;
   uint32_t* s_key = reinterpret_cast<uint32_t*>(s_tail + a.groups * step);  // [per_block + 2]: the keys before, in and behind the stretch
   uint32_t* s_pos = s_key + per_block + 2;          // [per_block]
   unsigned char* s_flag = reinterpret_cast<unsigned char*>(s_pos + per_block);  // [groups]
@@ -463,8 +510,8 @@ sum_kernel(SumArgs a, const T* __restrict__ grad) {
   const int r = threadIdx.x / a.group, lane = threadIdx.x - r * a.group;
   const int col = (blockIdx.y * a.group + lane) * N;
   const bool work = r < a.groups && col < a.dim;
-  float* head = s_head + r * step + lane * N;
-  float* tail = s_tail + r * step + lane * N;
+  Part<N>* head = s_head + r * step + lane * N;
+  Part<N>* tail = s_tail + r * step + lane * N;
   if (work) {
     const int q0 = r * a.per_group, q1 = q0 + a.per_group < count ? q0 + a.per_group : count;
     uint32_t flag = 0u;
@@ -480,25 +527,25 @@ sum_kernel(SumArgs a, const T* __restrict__ grad) {
   // block before.
   if (work) {
     const uint32_t own = s_flag[r];
-    float acc[N];
+    double acc[N];
     uint32_t flag = 0u;
     const int64_t slot = (int64_t)blockIdx.x * a.dim + col;
     if (r == 0 && (own & kHead)) {
-      nr_lds_get<N>(head, acc);
+      part_get<N>(head, acc);
       flag |= first_stop(s_span, 0, a.groups) < a.groups ? kHead : kHead | kSpan;
-      nr_store_some<float, N>(a.head + slot, a.dim - col, acc);
+      leave<N>(a.head + slot, a.dim - col, acc);
     }
     if (own & kTail) {
       const bool more = r + 1 < a.groups;
-      float next[N] = {};
-      nr_lds_get<N>(tail, acc);
-      if (more) nr_lds_get<N>(head + step, next);
+      double next[N] = {};
+      part_get<N>(tail, acc);
+      if (more) part_get<N>(head + step, next);
 #pragma unroll
       for (int k = 0; k < N; ++k) acc[k] += next[k];
       if (more && first_stop(s_span, r + 1, a.groups) < a.groups) {
         write_row<N>(a, s_key[(r + 1) * a.per_group], col, acc);
       } else {
-        nr_store_some<float, N>(a.tail + slot, a.dim - col, acc);
+        leave<N>(a.tail + slot, a.dim - col, acc);
         flag |= kTail;
       }
     }
@@ -538,6 +585,8 @@ constexpr int64_t kOwnTables = (int64_t)64 << 20;  // bytes of the chunks' table
                                                    // bf16 the sort's own traffic is half of that, 128 MB: 58 against 44
 constexpr int kCountSort = 256;  // lists up to this length: every entry counts the smaller ones
 constexpr int kOwnDigitBits = 9;  // (32 KB of counters)
+constexpr int kOwnPartBytes = 2 * kOwnThreads * 32;  // a lane's columns in two sums: 4 in 64 bits or 8 in 32
+static_assert(sizeof(Part<4>) * 4 == 32 && sizeof(Part<8>) * 8 == 32, "a lane's part of a sum");
 
 struct OwnArgs {
   SumArgs sum;
@@ -572,10 +621,10 @@ own_kernel(OwnArgs o, const T* __restrict__ grad, const I* __restrict__ idx) {
   if (gridDim.z > 1) a.out = static_cast<float*>(a.out) + (int64_t)blockIdx.z * a.rows * a.dim;  // (partial tables, in fp32)
   extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
   const int step = a.group * N, lane = nr_lane(), wave = threadIdx.x / NR_WAVE;
-  float* s_head = reinterpret_cast<float*>(lds);             // [groups][group * N]
-  float* s_tail = s_head + a.groups * step;
+  Part<N>* s_head = reinterpret_cast<Part<N>*>(lds);         // [groups][group * N]
+  Part<N>* s_tail = s_head + a.groups * step;
   uint32_t* s_digit = lds;                                   // [waves][512]: before the sums
-  uint32_t* s_list = lds + 2 * kOwnThreads * N;              // [chunk]
+  uint32_t* s_list = lds + kOwnPartBytes / 4;                // [chunk]
   uint32_t* s_named = s_list + o.chunk;                      // [named_words]: rows that have tokens, where they are cleared late
   unsigned char* s_flag = reinterpret_cast<unsigned char*>(s_named + o.named_words);  // [groups]
   __shared__ uint32_t s_count[kWaves];
@@ -735,8 +784,8 @@ own_kernel(OwnArgs o, const T* __restrict__ grad, const I* __restrict__ idx) {
   // the sums: the groups share the list evenly, a batch of loads at least
   const int share = (m + a.groups - 1) / a.groups, per = share > kFlight ? share : kFlight;
   auto key_at = [&](int q) { return q >= 0 && q < m ? s_list[q] >> kOwnPosBits : kNone; };
-  float* head = s_head + r * step + glane * N;
-  float* tail = s_tail + r * step + glane * N;
+  Part<N>* head = s_head + r * step + glane * N;
+  Part<N>* tail = s_tail + r * step + glane * N;
   const int q0 = r * per, q1 = q0 + per < m ? q0 + per : m;
   if (work) {
     uint32_t flag = 0u;
@@ -751,9 +800,9 @@ own_kernel(OwnArgs o, const T* __restrict__ grad, const I* __restrict__ idx) {
   __syncthreads();
   chain_heads<N>(s_span, r, work, a.groups, (m + per - 1) / per, s_head + glane * N, step);
   if (work && (s_flag[r] & kTail)) {  // (the last token's sum ends with the list: a group follows)
-    float acc[N], next[N];
-    nr_lds_get<N>(tail, acc);
-    nr_lds_get<N>(head + step, next);
+    double acc[N], next[N];
+    part_get<N>(tail, acc);
+    part_get<N>(head + step, next);
 #pragma unroll
     for (int k = 0; k < N; ++k) acc[k] += next[k];
     write_row<N>(a, (uint32_t)row0 + key_at(q1 - 1), col, acc);
@@ -767,7 +816,7 @@ merge_kernel(const float* __restrict__ tables, int chunks, int64_t elements, flo
   const int64_t i = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * 4;
   if (i >= elements) return;
   const int m = elements - i < 4 ? (int)(elements - i) : 4;
-  float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  double acc[4] = {0.0, 0.0, 0.0, 0.0};
   for (int c = 0; c < chunks; c += kFlight) {
     float x[kFlight][4];
 #pragma unroll
@@ -777,17 +826,12 @@ merge_kernel(const float* __restrict__ tables, int chunks, int64_t elements, flo
     for (int u = 0; u < kFlight; ++u)
       if (c + u < chunks)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) acc[k] += x[u][k];
+        for (int k = 0; k < 4; ++k) acc[k] += (double)x[u][k];
   }
+  float y[4];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) acc[k] *= scale;
-  if (accumulate) {
-    float was[4];
-    nr_load_some<O, 4>(out + i, m, was);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) acc[k] += was[k];
-  }
-  nr_store_some<O, 4>(out + i, m, acc);
+  for (int k = 0; k < 4; ++k) y[k] = (float)(acc[k] * (double)scale);
+  write_as<4, O>(out + i, m, accumulate != 0, y);
 }
 
 // A sum that starts in block b and leaves it: tail[b] + head[b + 1] + ... + the head that ends it.  A row that thousands of
@@ -802,7 +846,7 @@ join_kernel(SumArgs a, uint32_t blocks) {
   const uint32_t key = a.keys[(b + 1) * per_block < a.n ? (b + 1) * per_block - 1 : a.n - 1];
   if ((a.flags[b] & kTail) == 0u) return;
   __shared__ uint32_t s_end;
-  __shared__ float s_part[kJoinThreads * 4];
+  __shared__ double s_part[kJoinThreads * 4];
   if (threadIdx.x == 0) s_end = blocks;
   __syncthreads();
   for (uint32_t j0 = b + 1; j0 < blocks; j0 += kJoinThreads) {  // the first block from b + 1 on that ends the sum
@@ -822,9 +866,14 @@ join_kernel(SumArgs a, uint32_t blocks) {
   for (int col0 = 0; col0 < a.dim; col0 += lanes * 4) {
     const int col = col0 + lane * 4;
     const bool work = r < groups && col < a.dim;
-    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    double acc[4] = {0.0, 0.0, 0.0, 0.0};
     if (work) {
-      if (r == 0) nr_load_some<float, 4>(a.tail + (int64_t)b * a.dim + col, a.dim - col, acc);
+      if (r == 0) {
+        float tail[4];
+        nr_load_some<float, 4>(a.tail + (int64_t)b * a.dim + col, a.dim - col, tail);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[k] = (double)tail[k];
+      }
       const int h1 = (r + 1) * per < heads ? (r + 1) * per : heads;
       for (int h = r * per; h < h1; h += kFlight) {
         float x[kFlight][4];
@@ -835,7 +884,7 @@ join_kernel(SumArgs a, uint32_t blocks) {
         for (int u = 0; u < kFlight; ++u)
           if (h + u < h1)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) acc[k] += x[u][k];
+            for (int k = 0; k < 4; ++k) acc[k] += (double)x[u][k];
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k) s_part[(r * lanes + lane) * 4 + k] = acc[k];
@@ -995,7 +1044,7 @@ template <typename T>
 int launch_sum(const Plan& p, const SumArgs& a, const void* grad, hipStream_t stream) {
   constexpr int N = 16 / (int)sizeof(T);
   const int per_block = a.groups * a.per_group;
-  const size_t lds = (size_t)(2 * per_block + 2 + 2 * a.groups * a.group * N) * 4 + (size_t)(2 * a.groups);
+  const size_t lds = (size_t)(2 * per_block + 2) * 4 + (size_t)(2 * a.groups * a.group * N) * sizeof(Part<N>) + (size_t)(2 * a.groups);
   hipLaunchKernelGGL(sum_kernel<T>, dim3(p.sum_blocks, (uint32_t)p.col_tiles), dim3(kThreads), lds, stream, a, static_cast<const T*>(grad));
   NR_LAUNCH_CHECK();
   hipLaunchKernelGGL(join_kernel, dim3(p.sum_blocks), dim3(kJoinThreads), 0, stream, a, p.sum_blocks);
@@ -1003,24 +1052,20 @@ int launch_sum(const Plan& p, const SumArgs& a, const void* grad, hipStream_t st
   return 0;
 }
 
-constexpr size_t own_lds(int vec, int list_words, int named_words) {
-  return (size_t)(2 * kOwnThreads * vec + list_words + named_words) * 4 + kOwnThreads;
-}
+constexpr size_t own_lds(int list_words, int named_words) { return kOwnPartBytes + (size_t)(list_words + named_words) * 4 + kOwnThreads; }
 
 template <typename T, typename I>
 int launch_own(const OwnPlan& p, const OwnArgs& o, const void* grad, const void* idx, hipStream_t stream) {
-  constexpr int N = 16 / (int)sizeof(T);
   hipLaunchKernelGGL((own_kernel<T, I>), dim3((uint32_t)p.ranges, (uint32_t)p.col_tiles, (uint32_t)p.chunks), dim3(kOwnThreads),
-                     own_lds(N, o.chunk, o.named_words), stream, o, static_cast<const T*>(grad), static_cast<const I*>(idx));
+                     own_lds(o.chunk, o.named_words), stream, o, static_cast<const T*>(grad), static_cast<const I*>(idx));
   NR_LAUNCH_CHECK();
   return 0;
 }
 
 template <typename T>
 int init_own() {
-  constexpr int N = 16 / (int)sizeof(T);
-  if (int rc = nr_raise_lds(own_kernel<T, int64_t>, own_lds(N, kOwnMax, kOwnRangeMax / 32))) return rc;
-  return nr_raise_lds(own_kernel<T, int32_t>, own_lds(N, kOwnMax, kOwnRangeMax / 32));
+  if (int rc = nr_raise_lds(own_kernel<T, int64_t>, own_lds(kOwnMax, kOwnRangeMax / 32))) return rc;
+  return nr_raise_lds(own_kernel<T, int32_t>, own_lds(kOwnMax, kOwnRangeMax / 32));
 }
 
 template <typename O>

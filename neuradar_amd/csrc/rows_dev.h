@@ -134,19 +134,4 @@ __device__ __forceinline__ void nr_store_some(T* __restrict__ p, int m, const fl
   if (sizeof(T) == 2 && (bytes & 2)) *reinterpret_cast<typename NrPiece<uint16_t, T>::type*>(at) = (uint16_t)low;
 }
 
-// N floats in LDS, 16-byte aligned
-template <int N>
-__device__ __forceinline__ void nr_lds_get(const float* p, float (&x)[N]) {
-#pragma unroll
-  for (int q = 0; q < N / 4; ++q) {
-    const float4 v = reinterpret_cast<const float4*>(p)[q];
-    x[q * 4] = v.x; x[q * 4 + 1] = v.y; x[q * 4 + 2] = v.z; x[q * 4 + 3] = v.w;
-  }
-}
-template <int N>
-__device__ __forceinline__ void nr_lds_put(float* p, const float (&x)[N]) {
-#pragma unroll
-  for (int q = 0; q < N / 4; ++q) reinterpret_cast<float4*>(p)[q] = make_float4(x[q * 4], x[q * 4 + 1], x[q * 4 + 2], x[q * 4 + 3]);
-}
-
 }  // namespace

@@ -780,7 +780,7 @@ def embedding_grad(grad: Tensor, idx: Tensor, num_rows: int, scale: float = 1.0,
                    out: Optional[Tensor] = None, accumulate: bool = False, dtype: Optional[torch.dtype] = None) -> Tensor:
     """Gradient of `embedding` for its table: [num_rows, dim] with scale * (sum of grad[i] over idx[i] == v) in row v, by sorted
     indices -- no atomics, the same bits on every call.  grad [*idx.shape, dim] (rows may be apart), fp32 / bf16 / fp16; sums in
-    fp32, rounded once to the result's type (`dtype`; grad's own by default).
+    64 bits (fp32 between blocks), rounded to the result's type (`dtype`; grad's own by default).
     out: contiguous [num_rows, dim] that takes the result; accumulate: added to what `out` holds (rows that no index names are not
     touched).  Indices equal to padding_idx or outside [0, num_rows) contribute nothing.  Not differentiable: grad or out that autograd
     follows are refused (under torch.no_grad() they are not)."""
