@@ -266,8 +266,8 @@ _tensors = None
 
 
 def tensors() -> ctypes.PyDLL:
-    """libneuradar_tensors.so: nr_tensor_list, nr_mark_written and nr_shared_memory (csrc/tensor_list.cpp), called with the
-    interpreter lock held."""
+    """libneuradar_tensors.so: nr_tensor_list, nr_mark_written, nr_shared_memory and nr_clip_lists (csrc/tensor_list.cpp),
+    called with the interpreter lock held."""
     global _tensors
     if _tensors is None:
         if not os.path.exists(TENSORS_PATH):
@@ -276,6 +276,7 @@ def tensors() -> ctypes.PyDLL:
         handle.nr_tensor_list.argtypes = [ctypes.py_object, P, P, P]
         handle.nr_mark_written.argtypes = [ctypes.py_object]
         handle.nr_shared_memory.argtypes = [P, P, P, P, P, L]
+        handle.nr_clip_lists.argtypes = [ctypes.py_object, ctypes.py_object, P]
         _tensors = handle
     return _tensors
 

@@ -97,11 +97,37 @@ extern "C" int nr_shared_memory(const int64_t* src, const int32_t* src_dtype, co
     for (int64_t i = 0; i < n; ++i) {  // (the ranges of out are apart, so their ends ascend too: the first that ends behind r's start)
       if (numel[i] <= 0 || (src[i] == dst[i] && src_dtype[i] == dst_dtype[i])) continue;
       const Range r = range_of(src, numel, src_dtype, i);
+      if (r.to <= out.front().from || r.from >= out.back().to) continue;  // (all of them beside a bucket)
       const auto at = std::upper_bound(out.begin(), out.end(), r.from, [](uint64_t a, const Range& o) { return a < o.to; });
       if (at != out.end() && at->from < r.to) return kWrittenAndRead;
     }
     return kApart;
   } catch (...) {
     return kFailed;
+  }
+}
+
+// All that clipping asks of its two lists (or of one, in place), in one call: block <- [address n | elements n | place's address n | type n
+// (int32) | place's type n (int32)].  Returns the device and marks the places as written if nothing stands against taking the lists as
+// they are; else kNotTensors, without a mark: the caller finds out what with the functions above.
+extern "C" int nr_clip_lists(PyObject* grads, PyObject* outs, int64_t* block) {
+  try {
+    const int64_t n = (int64_t)PyList_GET_SIZE(grads);
+    if ((int64_t)PyList_GET_SIZE(outs) != n) return kNotTensors;
+    int64_t *numel = block + n, *dst = block + 2 * n;
+    int32_t *type = reinterpret_cast<int32_t*>(block + 3 * n), *dst_type = type + n;
+    const int device = nr_tensor_list(grads, block, numel, type);
+    if (device < 0) return kNotTensors;
+    if (outs == grads) {
+      std::copy(block, block + n, dst);
+      std::copy(type, type + n, dst_type);
+    } else {
+      std::vector<int64_t> count((size_t)n);
+      if (nr_tensor_list(outs, dst, count.data(), dst_type) != device || !std::equal(count.begin(), count.end(), numel)) return kNotTensors;
+    }
+    if (nr_shared_memory(block, type, dst, dst_type, numel, n) != kApart || nr_mark_written(outs) != 0) return kNotTensors;
+    return device;
+  } catch (...) {
+    return kNotTensors;
   }
 }

@@ -784,7 +784,8 @@ def embedding_grad(grad: Tensor, idx: Tensor, num_rows: int, scale: float = 1.0,
     out: contiguous [num_rows, dim] that takes the result; accumulate: added to what `out` holds (rows that no index names are not
     touched).  Indices equal to padding_idx or outside [0, num_rows) contribute nothing.  Not differentiable: grad or out that autograd
     follows are refused (under torch.no_grad() they are not)."""
-    if _differentiated(grad) or (out is not None and _differentiated(out)):
+    given = out is not None
+    if ((grad.requires_grad or forward_ad._current_level >= 0 or given) and (_differentiated(grad) or (given and _differentiated(out)))):
         raise RuntimeError("embedding_grad has no derivative: call it under torch.no_grad() or on detached tensors")
     device = grad.get_device()
     if device >= 0 and device != _current_device():
@@ -796,8 +797,7 @@ def embedding_grad(grad: Tensor, idx: Tensor, num_rows: int, scale: float = 1.0,
     grad = _float_rows(grad if grad.dim() == 2 else grad.reshape(n, dim), "grad")
     idx = _row_index(idx, device)
     padding = _padding_row(padding_idx, num_rows)
-    given = out is not None
-    if out is None:
+    if not given:
         if accumulate:
             raise RuntimeError("accumulate=True adds to `out`: give it")
         if dtype is not None and dtype not in _DTYPE_CODES:
@@ -853,7 +853,7 @@ def embedding(table: Tensor, idx: Tensor, scale: float = 1.0, padding_idx: Optio
     _float_rows(table, "table")
     idx = _row_index(idx, table.get_device())
     _padding_row(padding_idx, table.shape[0])
-    if _differentiated(table):  # (forward mode raises in there: there is no formula for it)
+    if (table.requires_grad or forward_ad._current_level >= 0) and _differentiated(table):  # (forward mode raises in there: there is no formula for it)
         return _Embedding.apply(table, idx, float(scale), padding_idx)
     return _embedding_rows(table, idx, float(scale))
 
@@ -1345,12 +1345,14 @@ _NORM_TYPES = {2.0: 2, 1.0: 1, float("inf"): 0}
 
 
 class _GradList:
-    """Addresses, sizes and types of a list of dense tensors as the host arrays that nr_grad_norm / nr_grad_scale read."""
+    """Addresses, sizes and types of a list of dense tensors as the host arrays that nr_grad_norm / nr_grad_scale read: one block,
+    [address n | elements n | type n (int32)], and where its three parts start."""
 
     def __init__(self, tensors: List[Tensor], what: str) -> None:
         self.count = n = len(tensors)
-        self.ptrs, self.numel, self.dtypes = array("q", bytes(8 * n)), array("q", bytes(8 * n)), array("i", bytes(4 * n))
-        self.arrays = self.ptrs.buffer_info()[0], self.numel.buffer_info()[0], self.dtypes.buffer_info()[0]
+        self.block = array("q", bytes(16 * n + (n + 1) // 2 * 8))
+        at = self.block.buffer_info()[0]
+        self.arrays = at, at + 8 * n, at + 16 * n
         self.tensors, self.plain = tensors, True
         self.device = _lib.tensors().nr_tensor_list(tensors, *self.arrays)
         if self.device == -4:
@@ -1365,6 +1367,25 @@ class _GradList:
                                .get(self.device, f"{what} cannot be read"))
 
 
+class _ClipLists:
+    """Gradients and places that are taken as they lie, for `_norm_and_factor`: (arrays, device) of nr_clip_lists' block."""
+    __slots__ = ("block", "count", "arrays", "device")
+
+    def __init__(self, block, count: int, arrays, device: int) -> None:
+        self.block, self.count, self.arrays, self.device = block, count, arrays, device
+
+    @classmethod
+    def read(cls, grads: List[Tensor], targets: List[Tensor]):
+        """(gradients, places), with the places marked as written; None if anything stands against it."""
+        n = len(grads)
+        block = array("q", bytes(32 * n))
+        at = block.buffer_info()[0]
+        device = _lib.tensors().nr_clip_lists(grads, targets, at)
+        if device < 0:
+            return None
+        return cls(block, n, (at, at + 8 * n, at + 24 * n), device), cls(block, n, (at + 16 * n, at + 8 * n, at + 28 * n), device)
+
+
 def _dense(t: Tensor) -> Tensor:
     """`t` itself if its elements fill a stretch of memory in some order of its dimensions (a channels-last weight), else a copy."""
     if t.layout != torch.strided:
@@ -1376,13 +1397,18 @@ def _dense(t: Tensor) -> Tensor:
     return p if p.is_contiguous() else t.contiguous()
 
 
-def _norm_and_factor(lst: _GradList, max_norm: float, norm_type: float, device, out: Optional[_GradList] = None) -> Tensor:
-    """[norm, clip factor, ...] on the device; with `out` the gradients clipped into it."""
+def _norm_kind(max_norm: float, norm_type: float) -> int:
     kind = _NORM_TYPES.get(float(norm_type))
     if kind is None:
         raise RuntimeError(f"norm_type must be 1, 2 or infinity, not {norm_type}")
     if not max_norm >= 0.0:
         raise RuntimeError(f"max_norm must not be negative or NaN: {max_norm}")
+    return kind
+
+
+def _norm_and_factor(lst: _GradList, max_norm: float, norm_type: float, device, out: Optional[_GradList] = None) -> Tensor:
+    """[norm, clip factor, ...] on the device; with `out` the gradients clipped into it."""
+    kind = _norm_kind(max_norm, norm_type)
     lib = _lib.lib()
     ptrs, numel, dtypes = lst.arrays
     need = lib.nr_grad_norm_workspace_bytes(numel, lst.count)
@@ -1446,29 +1472,34 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> Tens
     if device.type == "cuda" and device.index != _current_device():
         with torch.cuda.device(device):
             return clip_grads(grads, max_norm, norm_type, None if out is None else targets)
-    src = dst = _GradList(grads, "gradients")
+    max_norm = float(max_norm)
+    _norm_kind(max_norm, norm_type)
+    lists = _ClipLists.read(grads, targets)
+    if lists is not None:
+        return _norm_and_factor(lists[0], max_norm, norm_type, device, lists[1])[0]
+    src = dst = _GradList(grads, "gradients")  # something is refused, or has to be copied
     if out is not None:
         dst = _GradList(targets, "out")
         if dst.device != src.device:
             raise RuntimeError("out must be on the gradients' device")
-        if dst.numel != src.numel:
+        if dst.block[len(grads):2 * len(grads)] != src.block[len(grads):2 * len(grads)]:
             raise RuntimeError("out must hold one tensor of the same size for each gradient")
         if not (src.plain and dst.plain):  # elements are matched by place in memory: bring both into the order of their shapes
             if any(o.shape != g.shape for o, g in zip(targets, grads)):
                 raise RuntimeError("out must have its gradients' shapes where one of the two is not contiguous")
             src = _GradList([g.contiguous() for g in grads], "gradients")
             dst = _GradList([o if o.is_contiguous() else torch.empty_like(o, memory_format=torch.contiguous_format) for o in targets], "out")
-    shared = _lib.tensors().nr_shared_memory(src.arrays[0], src.arrays[2], dst.arrays[0], dst.arrays[2], src.arrays[1], src.count)
-    moved = not dst.plain or dst.tensors is not targets
+    shared, moved = 0, not dst.plain or dst.tensors is not targets
     if moved:
-        starts = [t.data_ptr() for t in targets if t.numel() > 0]
-        shared = shared or int(len(set(starts)) < len(starts))
         if any(s == 0 and n > 1 for t in targets for s, n in zip(t.stride(), t.shape)):
             raise RuntimeError("a tensor to be written holds several of its elements in one place")
+        starts = [t.data_ptr() for t in targets if t.numel() > 0]
+        shared = int(len(set(starts)) < len(starts))
+    shared = shared or _lib.tensors().nr_shared_memory(src.arrays[0], src.arrays[2], dst.arrays[0], dst.arrays[2], src.arrays[1], src.count)
     if shared != 0:
         raise RuntimeError("a tensor to be written is listed twice, or shares memory with another" if shared == 1 else
                            "a tensor to be written shares memory with a gradient (in place it has to be that gradient, in its own type)")
-    result = _norm_and_factor(src, float(max_norm), norm_type, device, dst)
+    result = _norm_and_factor(src, max_norm, norm_type, device, dst)
     _lib.tensors().nr_mark_written(targets)
     if moved:
         for target, written in zip(targets, dst.tensors):  # a target with holes gets its elements from a dense copy
