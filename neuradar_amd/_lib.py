@@ -7,6 +7,7 @@ __graft_entry__ as g; g.build()"` or `make -C neuradar_amd/csrc`).
 import ctypes
 import os
 import subprocess
+import sys
 from ctypes import POINTER, Structure, c_char_p, c_double, c_float, c_int, c_int64, c_uint32, c_void_p
 
 CSRC = os.path.join(os.path.dirname(os.path.abspath(__file__)), "csrc")
@@ -225,15 +226,35 @@ _lib = None
 def build(force: bool = False) -> str:
     """Compile the HIP library for gfx950 in-tree (hipcc cross-compiles without a GPU).  force: every file, whatever is built."""
     if force or not os.path.exists(LIB_PATH) or not os.path.exists(TENSORS_PATH) or _stale():
-        subprocess.check_call(["make", "-C", CSRC, "-j8"] + (["-B"] if force else []), stdout=subprocess.DEVNULL)
+        # (one after the other: whatever becomes of the second, which needs torch's headers, the kernels are built)
+        for target, all_of_it in (("libneuradar_hip.so", force), ("libneuradar_tensors.so", force or _other_torch())):
+            subprocess.check_call(["make", "-C", CSRC, "-j8", f"PYTHON={sys.executable}", target] + (["-B"] if all_of_it else []),
+                                  stdout=subprocess.DEVNULL)
     return LIB_PATH
 
 
+def built_for() -> str:
+    """What libneuradar_tensors.so has to be compiled against for this process."""
+    import torch
+
+    return "torch %s python %d.%d" % (torch.__version__, *sys.version_info[:2])
+
+
 def _stale() -> bool:
-    so = min(os.path.getmtime(LIB_PATH), os.path.getmtime(TENSORS_PATH))
     inc = os.path.join(os.path.dirname(CSRC), "..", "include", "neuradar_hip.h")
-    srcs = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".hip", ".h", ".cpp"))] + [inc]
-    return any(os.path.getmtime(s) > so for s in srcs if os.path.exists(s))
+    for built, ends, others in ((LIB_PATH, (".hip", ".h"), [inc]), (TENSORS_PATH, (".cpp",), [])):
+        srcs = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(ends)] + others
+        if any(os.path.getmtime(s) > os.path.getmtime(built) for s in srcs if os.path.exists(s)):
+            return True
+    return _other_torch()
+
+
+def _other_torch() -> bool:
+    """Whether libneuradar_tensors.so is there and compiled for another torch or Python than this process has."""
+    if not os.path.exists(TENSORS_PATH):
+        return False
+    with open(TENSORS_PATH, "rb") as f:
+        return built_for().encode() + b"\0" not in f.read()
 
 
 def lib() -> ctypes.CDLL:
@@ -273,6 +294,10 @@ def tensors() -> ctypes.PyDLL:
         if not os.path.exists(TENSORS_PATH):
             raise RuntimeError(f"{TENSORS_PATH} is missing. Build it with `make -C neuradar_amd/csrc`.")
         handle = ctypes.PyDLL(TENSORS_PATH)
+        handle.nr_built_for.restype = c_char_p
+        if handle.nr_built_for().decode() != built_for():
+            raise RuntimeError(f"{TENSORS_PATH} was built for {handle.nr_built_for().decode()}, this is {built_for()}: build it again "
+                               "(`make -C neuradar_amd/csrc -B libneuradar_tensors.so`)")
         handle.nr_tensor_list.argtypes = [ctypes.py_object, P, P, P]
         handle.nr_mark_written.argtypes = [ctypes.py_object]
         handle.nr_shared_memory.argtypes = [P, P, P, P, P, L]

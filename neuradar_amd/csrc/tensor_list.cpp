@@ -12,6 +12,9 @@ namespace {
 enum { kNotTensors = -1, kType = -2, kDevice = -3, kLayout = -4, kFailed = -5, kTracked = -6 };
 }
 
+// "torch V python X.Y": what this library was compiled against, and the only ones it may be loaded beside.
+extern "C" const char* nr_built_for() { return NR_BUILT_FOR; }
+
 // ptr, numel [len(list)], dtype [len(list)] (NR_DTYPE_*) <- the list's.  Returns the one device that they are on; or kNotTensors;
 // kType: one is not fp32 / bf16 / fp16; kTracked: autograd follows one, backwards or forwards; kDevice: not all on one GPU; kLayout:
 // one is not contiguous (its address is not taken).
