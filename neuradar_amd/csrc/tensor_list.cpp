@@ -17,7 +17,7 @@ extern "C" const char* nr_built_for() { return NR_BUILT_FOR; }
 
 // ptr, numel [len(list)], dtype [len(list)] (NR_DTYPE_*) <- the list's.  Returns the one device that they are on; or kNotTensors;
 // kType: one is not fp32 / bf16 / fp16; kTracked: autograd follows one, backwards or forwards; kDevice: not all on one GPU; kLayout:
-// one is not contiguous (its address is not taken).
+// one is not contiguous, or holds its values negated (its address is not taken).
 extern "C" int nr_tensor_list(PyObject* list, int64_t* ptr, int64_t* numel, int32_t* dtype) {
   try {
     if (!PyList_Check(list)) return kNotTensors;
@@ -39,7 +39,7 @@ extern "C" int nr_tensor_list(PyObject* list, int64_t* ptr, int64_t* numel, int3
       if (!t.is_cuda() || (device >= 0 && t.get_device() != device)) return kDevice;
       device = (int)t.get_device();
       numel[i] = t.numel();
-      if (t.layout() != at::kStrided || !t.is_contiguous()) dense = false;
+      if (t.layout() != at::kStrided || !t.is_contiguous() || t.is_neg()) dense = false;
       else ptr[i] = numel[i] > 0 ? reinterpret_cast<int64_t>(t.data_ptr()) : 0;
     }
     return dense ? device : kLayout;

@@ -746,8 +746,8 @@ def _padding_row(padding_idx: Optional[int], rows: int) -> int:
 
 def _strided_rows(t: Tensor) -> Tuple[Tensor, int]:
     """[n, dim] as (tensor, elements between rows) with neighbouring columns: a copy only where the columns are apart."""
-    if (t.shape[1] > 1 and t.stride(1) != 1) or t.stride(0) < 0:
-        t = t.contiguous()
+    if t.is_neg() or (t.shape[1] > 1 and t.stride(1) != 1):
+        t = t.resolve_neg().contiguous()
     return t, t.stride(0)
 
 
@@ -803,7 +803,7 @@ def embedding_grad(grad: Tensor, idx: Tensor, num_rows: int, scale: float = 1.0,
         if dtype is not None and dtype not in _DTYPE_CODES:
             raise RuntimeError(f"dtype must be float32, bfloat16 or float16, not {dtype}")
         out = grad.new_empty((num_rows, dim), dtype=dtype)
-    elif (_float_rows(out, "out").shape != (num_rows, dim) or not out.is_contiguous() or out.get_device() != device
+    elif (_float_rows(out, "out").shape != (num_rows, dim) or not out.is_contiguous() or out.is_neg() or out.get_device() != device
           or dtype not in (None, out.dtype)):
         raise RuntimeError(f"out must be a contiguous [{num_rows}, {dim}] tensor on grad's device" + ("" if dtype is None else f" of {dtype}"))
     grad, stride = _strided_rows(grad)
@@ -1390,6 +1390,7 @@ def _dense(t: Tensor) -> Tensor:
     """`t` itself if its elements fill a stretch of memory in some order of its dimensions (a channels-last weight), else a copy."""
     if t.layout != torch.strided:
         raise RuntimeError("sparse gradients are not supported")
+    t = t.resolve_neg()  # (a view that holds its values negated: the kernels read what lies there)
     if t.is_contiguous():
         return t
     order = sorted(range(t.dim()), key=lambda d: -t.stride(d))
@@ -1487,8 +1488,8 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> Tens
         if not (src.plain and dst.plain):  # elements are matched by place in memory: bring both into the order of their shapes
             if any(o.shape != g.shape for o, g in zip(targets, grads)):
                 raise RuntimeError("out must have its gradients' shapes where one of the two is not contiguous")
-            src = _GradList([g.contiguous() for g in grads], "gradients")
-            dst = _GradList([o if o.is_contiguous() else torch.empty_like(o, memory_format=torch.contiguous_format) for o in targets], "out")
+            src = _GradList([g.resolve_neg().contiguous() for g in grads], "gradients")
+            dst = _GradList([o if o.is_contiguous() and not o.is_neg() else torch.empty_like(o, memory_format=torch.contiguous_format) for o in targets], "out")
     shared, moved = 0, not dst.plain or dst.tensors is not targets
     if moved:
         if any(s == 0 and n > 1 for t in targets for s, n in zip(t.stride(), t.shape)):
@@ -1503,7 +1504,7 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> Tens
     _lib.tensors().nr_mark_written(targets)
     if moved:
         for target, written in zip(targets, dst.tensors):  # a target with holes gets its elements from a dense copy
-            if written.data_ptr() != target.data_ptr():
+            if written is not target and (written.data_ptr() != target.data_ptr() or target.is_neg()):
                 target.copy_(written)
     return result[0]
 

@@ -137,3 +137,15 @@ def test_norm_workspace_and_result():
                 rc = lib.nr_grad_norm(lst.arrays[0], lst.arrays[1], lst.arrays[2], lst.count, 2, 0.5, result.data_ptr(), ws.data_ptr(), st)
             assert rc == 0 and untouched(buf, result) and bool((ws[need:] == 0xA5).all()), sizes
             assert torch.equal(result[0], ops.grad_norm(grads)), sizes
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
+@pytest.mark.parametrize("n,rows", [(20, 3), (17000, 2), (17000, 700)])
+def test_widest_rows(n, rows, dtype):
+    """65 536 columns, the widest row there is, in each of the three ways; one row of gradient stands for all (stride 0), whole numbers."""
+    gen = torch.Generator().manual_seed(n)
+    idx, row = indices(n, rows, gen), torch.randint(-2, 3, (1, 65536), generator=gen).to(dtype).to(DEV)
+    buf, part = place(rows * 65536, F32, 3)
+    ops.embedding_grad(row.expand(n, 65536), idx, rows, out=part.view(rows, 65536))
+    assert untouched(buf, part)
+    assert torch.equal(part.view(rows, 65536), torch.bincount(idx, minlength=rows)[:, None].float() * row.float())
