@@ -19,9 +19,9 @@
 //     group, one that leaves the block is left in the workspace and added up in block order by a last launch.
 // Bound by memory where rows are long (read g once, write the table once), by the chain of launches and of dependent steps inside
 // a block where they are few.  Measured, kernels alone: rows 262 144 x 1 024 bf16 114 us (0.69 GB of traffic: 6.0 TB/s; 153 us on
-// a cold table); gradient 16 384 x 16 on 60 rows 11 us, 113 840 x 32 on 1 999 rows 18 + 4, 8 192 x 8 on 2^22 rows 25 (134 MB of
-// zeros alone: 18), 100 003 x 257 on 7 rows 32 + 4 (103 MB: 20), 131 072 x 512 bf16 on 131 072 rows 108 (sort 45, which also
-// writes the zeros; sums 53 at 3.2 TB/s; join 9).
+// a cold table); gradient 16 384 x 16 on 60 rows 11 us, 113 840 x 32 on 1 999 rows 19 + 4, 8 192 x 8 on 2^22 rows 26 (134 MB of
+// zeros alone: 18), 100 003 x 257 on 7 rows 33 + 4 (103 MB: 20), 131 072 x 512 bf16 on 131 072 rows 109 (sort 45, which also
+// writes the zeros; sums 54 at 3.2 TB/s; join 9).
 #include <type_traits>
 
 #include "rows_dev.h"
@@ -151,8 +151,8 @@ sort_count_kernel(SortPass s, const I* __restrict__ idx) {
   for (int d = threadIdx.x; d < digits; d += kThreads) s.counts[(int64_t)blockIdx.x * digits + d] = cnt[d];
 }
 
-// counts[b][d] -> tokens of digit d in blocks before b; totals[d].  A wave takes 16 digits and a quarter of the blocks for each
-// (lanes of one quarter read neighbouring digits), the quarters are then shifted by what lies before them.
+// counts[b][d] -> tokens of digit d in blocks before b; totals[d].  A block takes 16 digits; 16 threads, one per digit, walk a
+// sixteenth of the sort's blocks (neighbouring threads read neighbouring digits), the parts are then shifted by what lies before them.
 constexpr int kScanDigits = 16;
 __global__ void __launch_bounds__(kThreads)
 sort_scan_kernel(SortPass s) {
@@ -917,8 +917,8 @@ struct Plan {
   int64_t off_pairs, off_counts, off_totals, off_flags, off_parts, bytes;
 };
 
-// Everything that follows from the sizes: the digits of the sort, the stretches of the sum and the workspace.  The layout takes
-// the narrower vector (4 columns per lane): one size for every type of gradient.
+// Everything that follows from the sizes and from the gradient's element size, which sets the columns of a lane: the digits of the
+// sort, the stretches of the sum and the workspace.
 Plan make_plan(int64_t rows, int dim, int64_t n, int elem_size) {
   Plan p = {};
   while ((rows >> p.bits) != 0) ++p.bits;  // keys 0 .. rows

@@ -9,8 +9,8 @@
 // fixed piece of it.  Every block leaves one partial result; one block adds those up in order: the same bits on every call.
 // Sums are held in fp64: a vector FMA in fp64 costs what one in fp32 does, and no square of an fp32 value over- or underflows in
 // it.  NaN and infinity travel as in torch: the maximum compares bit patterns of |x|, where NaN is the largest.
-// Measured: 153 M fp32 (613 MB) norm 95 us = 6.5 TB/s, finish 5 us, scaling into other buffers 214 us = 5.7 TB/s (a copy of this
-// size: 5.0); 288 bf16 tensors of 134 MB in all: 3 x 11 + 3 + 3 x 15 us; 24 small tensors: 3.9 + 1.6 us, two launches; 75 tensors of
+// Measured: 153 M fp32 (613 MB) norm 95 to 97 us = 6.4 TB/s, finish 5 us, scaling into other buffers 214 us = 5.7 TB/s (a copy of this
+// size: 5.0); 288 bf16 tensors of 134 MB in all: 3 x 10 + 3 + 3 x 15 us; 24 small tensors: 3.8 + 1.7 us, two launches; 75 tensors of
 // 1.8 MB clipped: 4.4 + 5.2 us, two launches.
 #include "rows_dev.h"
 
