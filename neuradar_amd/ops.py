@@ -846,8 +846,8 @@ class _Embedding(torch.autograd.Function):
 
 def embedding(table: Tensor, idx: Tensor, scale: float = 1.0, padding_idx: Optional[int] = None) -> Tensor:
     """scale * table[idx]: rows of an embedding table [rows, dim] (fp32 / bf16 / fp16; rows may be apart, columns neighbours) for
-    indices of any shape (int64 / int32) -> [*idx.shape, dim] in the table's type, one rounding.  An index outside [0, rows) gives
-    a row of NaN and no gradient (nothing is read on the host, so nothing can be raised).
+    indices of any shape (int64 / int32) -> [*idx.shape, dim] in the table's type (the product formed in fp32, then rounded).  An
+    index outside [0, rows) gives a row of NaN and no gradient (nothing is read on the host, so nothing can be raised).
     Differentiable in the table, backwards and once: embedding_grad, inside `direct_param_grads` straight into table.grad.
     padding_idx as in nn.Embedding: that row is looked up like any other and gets no gradient."""
     _float_rows(table, "table")
@@ -1368,7 +1368,7 @@ class _GradList:
 
 
 class _ClipLists:
-    """Gradients and places that are taken as they lie, for `_norm_and_factor`: (arrays, device) of nr_clip_lists' block."""
+    """Gradients, or their places, that are taken as they lie: what _norm_and_factor reads of a _GradList, in nr_clip_lists' block."""
     __slots__ = ("block", "count", "arrays", "device")
 
     def __init__(self, block, count: int, arrays, device: int) -> None:
@@ -1407,8 +1407,8 @@ def _norm_kind(max_norm: float, norm_type: float) -> int:
     return kind
 
 
-def _norm_and_factor(lst: _GradList, max_norm: float, norm_type: float, device, out: Optional[_GradList] = None) -> Tensor:
-    """[norm, clip factor, ...] on the device; with `out` the gradients clipped into it."""
+def _norm_and_factor(lst, max_norm: float, norm_type: float, device, out=None) -> Tensor:
+    """[norm, clip factor, ...] on the device; with `out` the gradients clipped into it.  lst, out: _GradList or _ClipLists."""
     kind = _norm_kind(max_norm, norm_type)
     lib = _lib.lib()
     ptrs, numel, dtypes = lst.arrays
@@ -1458,11 +1458,11 @@ def clip_factor(grads, max_norm: float, norm_type: float = 2.0) -> Tuple[Tensor,
 
 def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> Tensor:
     """Scale gradients by min(1, max_norm / (norm + 1e-6)), norm = grad_norm(grads, norm_type), which is returned.  In place, or
-    into the tensors of `out` (as many elements each, any of the three types: places in a 16-bit bucket, say), one rounding.
-    Nothing is read on the host; a norm of NaN makes every gradient NaN, as in torch.  Tensors that are written must not share
-    memory, neither with one another nor with a gradient other than their own in its own type: refused (of tensors with holes, those
-    that start at one address).  Not differentiable: tensors that autograd follows are refused (under
-    torch.no_grad() they are not); a graph that saved a tensor which is written here raises when it is differentiated."""
+    into the tensors of `out` (as many elements each, any of the three types: places in a 16-bit bucket, say); the product is
+    formed in fp32, then rounded.  Nothing is read on the host; a norm of NaN makes every gradient NaN, as in torch.
+    Tensors that are written must not share memory, neither with one another nor with a gradient other than their own in its own
+    type: refused (of tensors with holes, those that start at one address).  Not differentiable: tensors that autograd follows are
+    refused (under torch.no_grad() they are not); a graph that saved a tensor which is written here raises when it is differentiated."""
     grads = _as_list(grads)
     targets = grads if out is None else _as_list(out)
     if len(targets) != len(grads):
