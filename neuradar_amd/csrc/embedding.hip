@@ -648,7 +648,7 @@ own_kernel(OwnArgs o, const T* __restrict__ grad, const I* __restrict__ idx) {
     item[u] = kNone;
     const int i = first + u * NR_WAVE;
     if (u < o.rounds) {
-      const uint64_t d = (uint64_t)((int64_t)raw[u] - row0);  // (below the range: far above it)
+      const uint64_t d = (uint64_t)(int64_t)raw[u] - (uint64_t)row0;  // (below the range: far above it; the lowest index of all, too)
       if (i < n && d < (uint64_t)range && (uint32_t)d != padding) item[u] = ((uint32_t)d << kOwnPosBits) | (uint32_t)i;
     }
   }

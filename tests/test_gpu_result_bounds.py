@@ -149,3 +149,34 @@ def test_widest_rows(n, rows, dtype):
     ops.embedding_grad(row.expand(n, 65536), idx, rows, out=part.view(rows, 65536))
     assert untouched(buf, part)
     assert torch.equal(part.view(rows, 65536), torch.bincount(idx, minlength=rows)[:, None].float() * row.float())
+
+
+@pytest.mark.parametrize("n,rows", [(16, 5), (3000, 70000), (17000, 60), (17000, 900000)])
+def test_indices_at_the_ends_of_their_types(n, rows):
+    """The lowest and highest values of the index types lie in no table: rows of NaN, and nothing of theirs in a gradient."""
+    gen = torch.Generator().manual_seed(n)
+    for itype in (torch.int32, torch.int64):
+        ends, inside = torch.iinfo(itype), torch.randint(0, rows, (n,), generator=gen)
+        idx = inside.to(itype)
+        far = torch.rand(n, generator=gen) < 0.3
+        values = torch.tensor([ends.min, ends.min + 1, ends.max, ends.max - 1, -1, rows], dtype=itype)
+        idx[far] = values[torch.randint(0, 6, (int(far.sum()),), generator=gen)]
+        grad = torch.randint(-2, 3, (n, 24), generator=gen).float()
+        want = torch.zeros(rows, 24).index_add_(0, inside[~far], grad[~far])
+        assert torch.equal(ops.embedding_grad(grad.to(DEV), idx.to(DEV), rows).cpu(), want), itype
+        table = torch.randn(rows, 24, generator=gen)
+        got = ops.embedding(table.to(DEV), idx.to(DEV)).cpu()
+        assert torch.equal(got[~far], table[inside[~far]]) and bool(torch.isnan(got[far]).all()), itype
+
+
+def test_norm_and_clip_of_a_tensor_beyond_32_bits():
+    x = torch.zeros((1 << 31) + 70001, device=DEV, dtype=BF16)
+    tail = torch.tensor([12.0], device=DEV)
+    x[0], x[-1] = -4.0, 3.0
+    assert float(ops.grad_norm([x, tail])) == 13.0 and float(ops.grad_norm([x], 1.0)) == 7.0 and float(ops.grad_norm([x], float("inf"))) == 4.0
+    out = torch.full((x.numel() + 1,), KNOWN, device=DEV, dtype=BF16)
+    ops.clip_grads([x, tail], 6.5, out=[out[:-1], torch.empty_like(tail)])
+    assert float(out[0]) == -2.0 and float(out[-2]) == 1.5 and float(out[-1]) == KNOWN and int(torch.count_nonzero(out[:-1])) == 2
+    ops.clip_grads([x, tail], 6.5)
+    assert float(x[0]) == -2.0 and float(x[-1]) == 1.5
+    assert abs(float(tail) - 6.0) <= 6.0 * (1e-6 / 13.0 + 2.0 ** -23)  # (the factor is 6.5 / (13 + 1e-6), rounded once, and its product once)
